@@ -219,6 +219,43 @@ size_t ifd_gemm_t64x8_w8a8_workspace(int M, int N, int K);
 int ifd_gemm_t64x8_w8a8(const int8_t* U, const float* XS, int per_token, const void* wt, int N, int K, void* C,
                         int ldc, int M, int mode, void* workspace, size_t ws_bytes, void* stream);
 
+/* ---- linears with an epilogue (no counterpart in the reference, whose linears have neither bias nor activation) --
+ * C = act(A . W^T + bias) + res, with the product's sums, the bias, the activation and the residual in fp32 and one
+ * rounding to C's type: bf16, or fp32 with out_f32 = 1. The products are those of ifd_gemm_t64 / ifd_gemm_t64x8 at the
+ * same sizes: weights s q + b up to 16 rows, each rounded to bf16 beyond (few column tiles: up to 64 rows unrounded).
+ * bias bf16 [N] or NULL. res bf16 [M][ldr] or NULL; it may be C itself (same pointer and stride, bf16 output: the residual
+ * stream updated in place), and must not overlap C otherwise. act: IFD_ACT_*:
+ *   RELU max(y, 0); SILU y / (1 + exp(-y)); GELU y Phi(y) (Phi the normal distribution's); GELU_TANH
+ *   y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))), the tanh form of the same.
+ * K % 256 == 0 (T64) or K % 64 == 0 (T64x8), lda % 8 == 0; A and wt 16-byte aligned; any N and ldc >= N. */
+enum { IFD_ACT_NONE = 0, IFD_ACT_RELU = 1, IFD_ACT_SILU = 2, IFD_ACT_GELU = 3, IFD_ACT_GELU_TANH = 4 };
+size_t ifd_gemm_t64_epi_workspace(int M, int N, int K);
+int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
+                     const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace, size_t ws_bytes,
+                     void* stream);
+size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K);
+int ifd_gemm_t64x8_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
+                       const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace,
+                       size_t ws_bytes, void* stream);
+
+/* ---- sampling from a head's logits (in the reference the host samples; here the logits stay on the device) --------
+ * One token per row of logits [T][ld] (fp32 as store mode 2 writes them, or bf16 with logits_bf16 = 1), V columns, from
+ * the row's random number u in [0, 1):
+ *   w_i = exp((l_i - max l) / temperature). In the order of falling logits (equal ones: rising index) are kept the
+ *   first top_k; of these the shortest prefix whose weights reach top_p times theirs all; of these the w_i >= min_p.
+ *   token = the first index, in the order of the vocabulary, at which the sum of kept weights exceeds u times their
+ *   total; prob = its weight over that total.
+ * temperature, top_p, min_p float [T] and top_k int [T], one value per row; NULL: off for every row. temperature <= 0
+ * (or NaN): the largest logit (equal ones: the lowest index), prob 1. top_k <= 0 or >= V, top_p >= 1, min_p <= 0: off;
+ * top_p <= 0 or NaN keeps one token, min_p > 1 counts as 1. u is taken into [0, 1 - 2^-24]. Logits of minus infinity
+ * (a grammar's mask) or NaN are never drawn; a row that has no others gets token -1 and prob 0. Plus infinity counts as a
+ * weight of 1 among zeros. Computed in 64 bits: weights below 2^-45 of the largest count as 0. prob may be NULL. */
+enum { IFD_SAMPLE_MAX_V = 1 << 19 };
+size_t ifd_sample_workspace(int T, int V);
+int ifd_sample(const void* logits, int logits_bf16, int T, int V, int ld, const float* temperature, const int* top_k,
+               const float* top_p, const float* min_p, const float* u, int* token, float* prob, void* workspace,
+               size_t ws_bytes, void* stream);
+
 /* ---- MoE (reference encode_moe sorted path, qwen35.h:1869-1980; kernels moe.metal:60-187) -------------------- */
 
 /* Router logits [T][E1] = x [T][H] . W [E1][H]^T, bf16 operands, fp32 accumulation; out_bf16 = 1 rounds to bf16
@@ -231,6 +268,23 @@ int ifd_moe_router_logits(const void* x, const void* w, int T, int H, int E1, in
  * shared_gate == 1, 1.0 when 0 (always-on shared expert). Ties go to the lowest expert index. E <= 512, k <= 16. */
 int ifd_moe_route(const void* logits, int logits_bf16, int T, int E, int k, int stride, int norm, int shared_gate,
                   int* idx, float* wt, float* sg, void* stream);
+
+/* Routing with sigmoid scores, a balance bias and expert groups (no counterpart in the reference, whose models route by
+ * softmax alone). Per token, over its logits l [E] (row stride `stride`):
+ *   s_e = softmax(l)_e (IFD_SCORE_SOFTMAX) or 1 / (1 + exp(-l_e)) (IFD_SCORE_SIGMOID)
+ *   c_e = s_e + bias_e, bias float [E]; with bias NULL the logits themselves are compared
+ *   groups > 1: the experts are that many runs of E / groups; a run's value is its largest c (group_top = 1) or the sum of
+ *   its two largest (group_top = 2; of s where bias is NULL), and only the topk_groups best runs stay
+ *   idx int [T][k]: the k largest c, falling; wt float [T][k]: s (without the bias), divided by the picks' sum when
+ *   norm != 0 (0 where that sum is 0), times scale; sg float [T] as in ifd_moe_route.
+ * Choices are made in 64 bits; ties go to the lowest index. NaN logits and biases count as minus infinity. An expert whose
+ * choice is minus infinity is picked only when its groups hold no others; a row of minus infinities has scores 0.
+ * E <= 512, k <= 16, groups <= 64 and a divisor of E, topk_groups runs hold at least k experts. idx, wt and sg feed
+ * ifd_moe_dispatch(_ex), ifd_moe_rows(_t64) and ifd_moe_combine. */
+enum { IFD_SCORE_SOFTMAX = 0, IFD_SCORE_SIGMOID = 1 };
+int ifd_moe_route_ex(const void* logits, int logits_bf16, int T, int E, int k, int stride, int score, const float* bias,
+                     int groups, int topk_groups, int group_top, int norm, float scale, int shared_gate, int* idx,
+                     float* wt, float* sg, void* stream);
 
 /* Stable counting sort of routed rows r = t*k + j by expert (reference moe_sort, moe.metal:130-161, whose order
  * inside a segment is atomic-order; this one keeps row order): offsets int [E+1], perm int [R] (sorted position ->

@@ -19,6 +19,7 @@ _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/inferd_qmm.h
 _GEMM_ARGS = [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _u32, _vp, _i, _i, _i, _vp, _sz, _vp]
+_EPI_ARGS = [_vp, _i, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _sz, _vp]
 SIGNATURES = {
     "ifd_version": (_i, []),
     "ifd_status_str": (ctypes.c_char_p, [_i]),
@@ -61,8 +62,15 @@ SIGNATURES = {
     "ifd_gemm_t64x8": (_i, [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _vp, _sz, _vp]),
     "ifd_gemm_t64x8_w8a8_workspace": (_sz, [_i, _i, _i]),
     "ifd_gemm_t64x8_w8a8": (_i, [_vp, _vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _vp, _sz, _vp]),
+    "ifd_gemm_t64_epi_workspace": (_sz, [_i, _i, _i]),
+    "ifd_gemm_t64_epi": (_i, _EPI_ARGS),
+    "ifd_gemm_t64x8_epi_workspace": (_sz, [_i, _i, _i]),
+    "ifd_gemm_t64x8_epi": (_i, _EPI_ARGS),
+    "ifd_sample_workspace": (_sz, [_i, _i]),
+    "ifd_sample": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ifd_moe_router_logits": (_i, [_vp, _vp, _i, _i, _i, _i, _vp, _vp]),
     "ifd_moe_route": (_i, [_vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "ifd_moe_route_ex": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _vp]),
     "ifd_moe_tiles_max": (_i, [_i, _i]),
     "ifd_moe_dispatch_workspace": (_sz, [_i, _i]),
     "ifd_moe_dispatch": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

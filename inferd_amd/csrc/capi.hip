@@ -1,6 +1,7 @@
 // The C ABI (include/inferd_qmm.h): argument checks, routing, workspace layout, and the one-shot MoE FFN.
 #include <algorithm>
 
+#include "epi.h"
 #include "host.h"
 #include "kernels.h"
 #include "t64.h"
@@ -378,6 +379,100 @@ int ifd_gemm_t64x8_w8a8(const int8_t* U, const float* XS, int per_token, const v
   return launch_w8a8_t(U, XS, wt, N, K, C, ldc, M, mode, w.body, w.bytes, S(stream));
 }
 
+// ---- linears with an epilogue --------------------------------------------------------------------------------------
+namespace {
+// The arguments that both layouts share.
+int check_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act, const void* res,
+              int ldr, const void* C, int ldc, int M, int out_f32, const void* workspace) {
+  IFD_CHECK(act >= IFD_ACT_NONE && act <= IFD_ACT_GELU_TANH, "act=%d must be one of IFD_ACT_*", act);
+  IFD_CHECK(out_f32 == 0 || out_f32 == 1, "out_f32=%d must be 0 or 1", out_f32);
+  IFD_CHECK(lda >= K && lda % 8 == 0 && ldc >= N && (!res || ldr >= N), "bad strides lda=%d ldc=%d ldr=%d", lda, ldc, ldr);
+  if (M == 0) return IFD_OK;
+  IFD_CHECK(A && wt && C && aligned(A, 16) && aligned(wt, 16), "null or misaligned pointer");
+  IFD_CHECK(aligned(C, out_f32 ? 4 : 2) && aligned(bias, 2) && aligned(res, 2), "misaligned C, bias or residual");
+  IFD_CHECK(!workspace || aligned(workspace, 16), "workspace must be 16-byte aligned");
+  if (res) {
+    const char *c = (const char*)C, *r = (const char*)res;
+    const size_t ce = ((size_t)(M - 1) * ldc + N) * (out_f32 ? 4 : 2), re = ((size_t)(M - 1) * ldr + N) * 2;
+    IFD_CHECK((c == r && ldc == ldr && !out_f32) || c + ce <= r || r + re <= c,
+              "the residual overlaps C without being C itself");
+  }
+  return IFD_OK;
+}
+// The product goes to the workspace in fp32, behind the GEMM's own: [gemm | y [M][N]].
+size_t epi_ws(size_t gemm, int M, int N) { return with_header(align_up(gemm, 256) + (size_t)M * N * sizeof(float)); }
+}  // namespace
+
+size_t ifd_gemm_t64_epi_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 256) return 0;
+  return epi_ws(M <= 16 ? qmv_t_workspace(M, N, K, 2) : gemm_t_workspace(M, N, K, 2), M, N);
+}
+
+int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
+                     const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace, size_t ws_bytes,
+                     void* stream) {
+  IFD_CHECK(M >= 0 && N > 0 && K > 0 && K % 256 == 0, "bad shape M=%d N=%d K=%d (K multiple of 256)", M, N, K);
+  IFD_TRY(check_epi(A, lda, wt, N, K, bias, act, res, ldr, C, ldc, M, out_f32, workspace));
+  if (M == 0) return IFD_OK;
+  const size_t need = ifd_gemm_t64_epi_workspace(M, N, K);
+  if (!workspace || ws_bytes < need)
+    return fail(IFD_ERR_WORKSPACE, "gemm_t64_epi needs %zu bytes of workspace, got %zu", need, ws_bytes);
+  const WsView w = ws_view(workspace, ws_bytes);
+  const size_t gemm = need - kWsHeader - (size_t)M * N * sizeof(float);
+  float* y = (float*)((char*)w.body + gemm);
+  IFD_TRY(M <= 16 ? launch_qmv_t((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.cnt, w.body, gemm, S(stream))
+                  : launch_gemm_t((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.body, gemm, S(stream)));
+  return launch_epi(y, M, N, Epi{bias, (const uint16_t*)res, ldr, act}, C, ldc, out_f32, S(stream));
+}
+
+size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 64) return 0;
+  return epi_ws(t64x8_qmv(M, K) ? qmv_t_workspace(M, N, K, 2, 8) : gemm_sk8_workspace(M, N, K), M, N);
+}
+
+int ifd_gemm_t64x8_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
+                       const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace,
+                       size_t ws_bytes, void* stream) {
+  IFD_CHECK(M >= 0 && N > 0 && K > 0 && K % 64 == 0, "bad shape M=%d N=%d K=%d (K multiple of 64)", M, N, K);
+  IFD_TRY(check_epi(A, lda, wt, N, K, bias, act, res, ldr, C, ldc, M, out_f32, workspace));
+  if (M == 0) return IFD_OK;
+  const size_t need = ifd_gemm_t64x8_epi_workspace(M, N, K);
+  if (!workspace || ws_bytes < need)
+    return fail(IFD_ERR_WORKSPACE, "gemm_t64x8_epi needs %zu bytes of workspace, got %zu", need, ws_bytes);
+  const WsView w = ws_view(workspace, ws_bytes);
+  const size_t gemm = need - kWsHeader - (size_t)M * N * sizeof(float);
+  float* y = (float*)((char*)w.body + gemm);
+  IFD_TRY(t64x8_qmv(M, K) ? launch_qmv_t8((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.cnt, w.body, gemm, S(stream))
+                          : launch_gemm_sk8((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.body, gemm, S(stream)));
+  return launch_epi(y, M, N, Epi{bias, (const uint16_t*)res, ldr, act}, C, ldc, out_f32, S(stream));
+}
+
+// ---- sampling --------------------------------------------------------------------------------------------------------
+size_t ifd_sample_workspace(int T, int V) {
+  if (T <= 0 || V <= 0 || V > IFD_SAMPLE_MAX_V) return 0;
+  return with_header(sample_workspace(T, V));
+}
+
+int ifd_sample(const void* logits, int logits_bf16, int T, int V, int ld, const float* temperature, const int* top_k,
+               const float* top_p, const float* min_p, const float* u, int* token, float* prob, void* workspace,
+               size_t ws_bytes, void* stream) {
+  IFD_CHECK(T >= 0 && V > 0 && V <= IFD_SAMPLE_MAX_V, "bad shape T=%d V=%d (V <= %d)", T, V, IFD_SAMPLE_MAX_V);
+  IFD_CHECK(ld >= V, "ld=%d must be >= V=%d", ld, V);
+  IFD_CHECK(logits_bf16 == 0 || logits_bf16 == 1, "logits_bf16=%d must be 0 or 1", logits_bf16);
+  if (T == 0) return IFD_OK;
+  IFD_CHECK(logits && u && token, "null pointer");
+  IFD_CHECK(aligned(logits, logits_bf16 ? 2 : 4) && aligned(temperature, 4) && aligned(top_k, 4) && aligned(top_p, 4) &&
+                aligned(min_p, 4) && aligned(u, 4) && aligned(token, 4) && aligned(prob, 4),
+            "misaligned pointer");
+  IFD_CHECK(!workspace || aligned(workspace, 16), "workspace must be 16-byte aligned");
+  const size_t need = ifd_sample_workspace(T, V);
+  if (need && (!workspace || ws_bytes < need))
+    return fail(IFD_ERR_WORKSPACE, "sample needs %zu bytes of workspace, got %zu", need, ws_bytes);
+  const WsView w = ws_view(workspace, ws_bytes);
+  return launch_sample(logits, logits_bf16, T, V, ld, temperature, top_k, top_p, min_p, u, token, prob, w.body, w.bytes,
+                       S(stream));
+}
+
 int ifd_moe_router_logits(const void* x, const void* w, int T, int H, int E1, int out_bf16, void* logits,
                           void* stream) {
   IFD_CHECK(T >= 0 && H > 0 && H % 64 == 0 && E1 > 0, "bad shape T=%d H=%d E1=%d (H multiple of 64)", T, H, E1);
@@ -391,6 +486,26 @@ int ifd_moe_route(const void* logits, int logits_bf16, int T, int E, int k, int 
   IFD_CHECK(stride >= E + (shared_gate ? 1 : 0), "stride=%d too small for E=%d (+ shared gate)", stride, E);
   IFD_CHECK(T == 0 || (logits && idx && wt && sg), "null pointer");
   return launch_moe_route(logits, logits_bf16, T, E, k, stride, norm, shared_gate, idx, wt, sg, S(stream));
+}
+
+int ifd_moe_route_ex(const void* logits, int logits_bf16, int T, int E, int k, int stride, int score, const float* bias,
+                     int groups, int topk_groups, int group_top, int norm, float scale, int shared_gate, int* idx,
+                     float* wt, float* sg, void* stream) {
+  IFD_CHECK(E > 0 && E <= 512 && k > 0 && k <= 16 && k <= E && T >= 0, "bad routing shape E=%d k=%d", E, k);
+  IFD_CHECK(stride >= E + (shared_gate ? 1 : 0), "stride=%d too small for E=%d (+ shared gate)", stride, E);
+  IFD_CHECK(score == IFD_SCORE_SOFTMAX || score == IFD_SCORE_SIGMOID, "score=%d must be one of IFD_SCORE_*", score);
+  IFD_CHECK(groups > 0 && groups <= 64 && E % groups == 0, "groups=%d must be 1 to 64 and divide E=%d", groups, E);
+  IFD_CHECK(topk_groups > 0 && topk_groups <= groups && (long)topk_groups * (E / groups) >= k,
+            "topk_groups=%d of %d groups of %d experts cannot give %d picks", topk_groups, groups, E / groups, k);
+  IFD_CHECK(group_top == 1 || (group_top == 2 && E / groups >= 2), "group_top=%d must be 1, or 2 with groups of 2 or more",
+            group_top);
+  IFD_CHECK(scale - scale == 0.f, "scale must be finite");
+  if (T == 0) return IFD_OK;
+  IFD_CHECK(logits && idx && wt && sg, "null pointer");
+  IFD_CHECK(aligned(logits, logits_bf16 ? 2 : 4) && aligned(bias, 4) && aligned(idx, 4) && aligned(wt, 4) && aligned(sg, 4),
+            "misaligned pointer");
+  return launch_moe_route_ex(logits, logits_bf16, T, E, k, stride, score == IFD_SCORE_SOFTMAX, bias, groups, topk_groups,
+                             group_top, norm, scale, shared_gate, idx, wt, sg, S(stream));
 }
 
 int ifd_moe_tiles_max(int R, int E) { return moe_tiles_max(R, E); }

@@ -133,7 +133,20 @@ size_t gemm_t_a8_least_workspace(int M, int N, int K, int mode);
 int launch_gemm_t_a8(const uint16_t* Ab, const float* sxT, int Mp, const void* wt, int N, int K, void* C, int ldc,
                      int M, int mode, void* ws, size_t ws_bytes, hipStream_t st);
 
+// The epilogue of a linear, act(y + bias) + residual (epi.h), as a pass over its fp32 product y [M][N].
+struct Epi;
+int launch_epi(const float* y, int M, int N, const Epi& e, void* C, int ldc, int out_f32, hipStream_t st);
+
+// Sampling (sample.hip): logits [T][ld] of V <= 1 << 19 columns; temperature, top_k, top_p, min_p and prob may be null.
+size_t sample_workspace(int T, int V);
+int launch_sample(const void* logits, int logits_bf16, int T, int V, int ld, const float* temperature, const int* top_k,
+                  const float* top_p, const float* min_p, const float* u, int* token, float* prob, void* ws,
+                  size_t ws_bytes, hipStream_t st);
+
 // MoE.
+int launch_moe_route_ex(const void* logits, int logits_bf16, int T, int E, int k, int stride, int softmax,
+                        const float* bias, int groups, int topk_groups, int group_top, int norm, float scale,
+                        int shared_gate, int* idx, float* wt, float* sg, hipStream_t st);
 int launch_router_logits(const uint16_t* x, const uint16_t* w, int T, int H, int E1, int out_bf16, void* logits,
                          hipStream_t st);
 int launch_moe_route(const void* logits, int logits_bf16, int T, int E, int k, int stride, int norm, int shared_gate,

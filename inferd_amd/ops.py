@@ -41,6 +41,36 @@ def workspace(nbytes: int, device) -> torch.Tensor:
     return buf
 
 
+def _workspace_here(nbytes: int, device) -> torch.Tensor:
+    """A zeroed uint8 workspace for one call on the current stream: cached per device and stream, and a fresh one inside
+    a graph capture, so that calls on two streams, or two captured graphs, never share one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    key = (str(device), _stream())
+    buf = _ws_cache.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = _ws_cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return buf
+
+
+def _want(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on_device(device, *tensors) -> None:
+    """Every tensor on `device`, which is the current one (the calls go to its current stream)."""
+    _want(device.type == "cuda" and device.index == torch.cuda.current_device(),
+          f"tensors on {device}, which is not the current device")
+    _want(all(t is None or t.device == device for t in tensors), "tensors on different devices")
+
+
+def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, name: str) -> None:
+    """None, or a tensor of this shape and type with adjacent values in a row."""
+    _want(t is None or (t.shape == shape and t.dtype == dtype), f"{name}: {shape} {dtype} wanted")
+    _want(t is None or t.shape[-1] == 1 or t.stride(-1) == 1, f"{name}: the values of a row must be adjacent")
+
+
 @dataclass
 class QLinear:
     """MLX affine group-64 linear [N, K]: wq int32 [N, K bits/32] (uint32 bit patterns), s/b bf16 [N, K/64];
@@ -200,6 +230,80 @@ def gemm_t64x8_w8a8(U: torch.Tensor, XS: torch.Tensor, W: T64x8Linear, C: Option
     return C
 
 
+# ---- linears with an epilogue ---------------------------------------------------------------------------------------
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _gemm_epi(name: str, A, W, bias, act, residual, C, fp32) -> torch.Tensor:
+    _want(A.dim() == 2 and A.dtype == torch.bfloat16 and A.shape[1] == W.K, f"A: bf16 [M, {W.K}] wanted")
+    M, N = A.shape[0], W.N
+    _on_device(A.device, W.wt, bias, residual, C)
+    _rows(A, (M, W.K), torch.bfloat16, "A")
+    _want(act in ACTS, f"act={act!r} must be one of {sorted(ACTS)}")
+    _rows(bias, (N,), torch.bfloat16, "bias")
+    _rows(residual, (M, N), torch.bfloat16, "residual")
+    if C is None:
+        C = torch.empty((M, N), dtype=torch.float32 if fp32 else torch.bfloat16, device=A.device)
+    out = torch.float32 if C.dtype == torch.float32 else torch.bfloat16
+    _rows(C, (M, N), out, "C")
+    step = lambda t: t.stride(0) if M > 1 else t.shape[1]  # noqa: E731
+    L = lib()
+    need = getattr(L, name + "_workspace")(M, N, W.K)
+    ws = _workspace_here(need, A.device) if need else None
+    check(getattr(L, name)(_p(A), step(A), _p(W.wt), N, W.K, _p(bias), ACTS[act], _p(residual),
+                           0 if residual is None else step(residual), _p(C), step(C), M, int(out == torch.float32), _p(ws),
+                           need, _stream()))
+    return C
+
+
+def gemm_t64_epi(A: torch.Tensor, W: T64Linear, bias: Optional[torch.Tensor] = None, act: str = "none",
+                 residual: Optional[torch.Tensor] = None, C: Optional[torch.Tensor] = None,
+                 fp32: bool = False) -> torch.Tensor:
+    """C = act(A . W^T + bias) + residual for T64 weights, rounded once to bf16 (or fp32: `fp32`, or a fp32 C).
+
+    bias bf16 [N], residual bf16 [M, N] (it may be C itself); act: none, relu, silu, gelu, gelu_tanh. A, C and the residual
+    may have rows further apart than they are long (A's a multiple of 8 values)."""
+    return _gemm_epi("ifd_gemm_t64_epi", A, W, bias, act, residual, C, fp32)
+
+
+def gemm_t64x8_epi(A: torch.Tensor, W: T64x8Linear, bias: Optional[torch.Tensor] = None, act: str = "none",
+                   residual: Optional[torch.Tensor] = None, C: Optional[torch.Tensor] = None,
+                   fp32: bool = False) -> torch.Tensor:
+    """gemm_t64_epi for T64x8 (8-bit) weights."""
+    return _gemm_epi("ifd_gemm_t64x8_epi", A, W, bias, act, residual, C, fp32)
+
+
+# ---- sampling ---------------------------------------------------------------------------------------------------------
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, outs: Optional[tuple] = None):
+    """The next token of every row of logits [T, V] (fp32 or bf16) by its random number u [T] in [0, 1): returns
+    (token int32 [T], prob fp32 [T]), written to `outs` when given.
+
+    temperature, top_p, min_p fp32 [T] and top_k int32 [T] hold a value per row; None is off for all rows
+    (temperature 0: greedy; top_k 0, top_p 1, min_p 0: off for that row). See ifd_sample for the rule."""
+    _want(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16), "logits: fp32 or bf16 [T, V] wanted")
+    T, V = logits.shape
+    _rows(logits, (T, V), logits.dtype, "logits")
+    for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32)):
+        _rows(t, (T,), dtype, name)
+    if outs is None:
+        outs = (torch.empty((T,), dtype=torch.int32, device=logits.device),
+                torch.empty((T,), dtype=torch.float32, device=logits.device))
+    token, prob = outs
+    _rows(token, (T,), torch.int32, "token")
+    _rows(prob, (T,), torch.float32, "prob")
+    _on_device(logits.device, u, temperature, top_k, top_p, min_p, token, prob)
+    need = lib().ifd_sample_workspace(T, V)
+    ws = _workspace_here(need, logits.device) if need else None
+    check(lib().ifd_sample(_p(logits), int(logits.dtype == torch.bfloat16), T, V, logits.stride(0) if T > 1 else V,
+                           _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(token), _p(prob), _p(ws), need,
+                           _stream()))
+    return token, prob
+
+
 @dataclass
 class MoeW:
     """Stacked experts [E, N, K] in the same affine layout (engine/src/moe.h:8-11), 4-bit (wq [E, N, K/8]) or 8-bit
@@ -327,6 +431,38 @@ def moe_route(logits: torch.Tensor, E: int, k: int, norm: bool = True, shared_ga
     sg = torch.empty((T,), dtype=torch.float32, device=logits.device)
     check(lib().ifd_moe_route(_p(logits), 1 if logits.dtype == torch.bfloat16 else 0, T, E, k, stride,
                               1 if norm else 0, 1 if shared_gate else 0, _p(idx), _p(wt), _p(sg), _stream()))
+    return idx, wt, sg
+
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route_ex(logits: torch.Tensor, E: int, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+                 groups: int = 1, topk_groups: int = 1, group_top: int = 1, norm: bool = True, scale: float = 1.0,
+                 shared_gate: bool = False, outs: Optional[tuple] = None):
+    """Routing by softmax or sigmoid scores with a balance bias (fp32 [E], for the choice only), expert groups of which the
+    topk_groups best stay, weights renormalised (norm) and scaled; see ifd_moe_route_ex for the rule. logits [T, >= E (+ 1
+    with shared_gate)] fp32 or bf16. Returns (idx int32 [T, k], wt fp32 [T, k], sg fp32 [T]), as moe_route, written to
+    `outs` when given."""
+    _want(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16), "logits: fp32 or bf16 [T, E] wanted")
+    _want(score in SCORES, f"score={score!r} must be one of {sorted(SCORES)}")
+    T, width = logits.shape
+    _want(width >= E + (1 if shared_gate else 0), f"logits: {width} columns for E={E} (+ shared gate)")
+    _rows(logits, (T, width), logits.dtype, "logits")
+    _rows(bias, (E,), torch.float32, "bias")
+    dev = logits.device
+    if outs is None:
+        outs = (torch.empty((T, k), dtype=torch.int32, device=dev), torch.empty((T, k), dtype=torch.float32, device=dev),
+                torch.empty((T,), dtype=torch.float32, device=dev))
+    idx, wt, sg = outs
+    _want(idx.shape == wt.shape == (T, k) and sg.shape == (T,) and idx.dtype == torch.int32
+          and wt.dtype == sg.dtype == torch.float32 and all(t.is_contiguous() for t in outs),
+          f"outs: contiguous int32 [{T}, {k}], fp32 [{T}, {k}] and fp32 [{T}] wanted")
+    _on_device(dev, bias, idx, wt, sg)
+    check(lib().ifd_moe_route_ex(_p(logits), int(logits.dtype == torch.bfloat16), T, E, k,
+                                 logits.stride(0) if T > 1 else width, SCORES[score], _p(bias), groups,
+                                 topk_groups, group_top, int(norm), float(scale), int(shared_gate), _p(idx), _p(wt),
+                                 _p(sg), _stream()))
     return idx, wt, sg
 
 

@@ -1,0 +1,432 @@
+"""GPU checks of the epilogue linears, the extended routing and the sampling against plain implementations in 64 bits, one
+operator at a time and as the run of a decode step that they are used in."""
+import math
+
+import numpy as np
+import pytest
+
+from tests import gen
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}  # a rounding, relative
+
+
+def _gu():
+    from tests import gpu_util
+    return gpu_util
+
+
+def _ops():
+    from inferd_amd import ops
+    return ops
+
+
+# ---- routing ---------------------------------------------------------------------------------------------------------
+def plain_route(logits, E, k, score, bias, groups, topk_groups, group_top, norm, scale, gate):
+    """ifd_moe_route_ex's rule, row by row in 64 bits."""
+    idx, wt, sg = [], [], []
+    for row in logits.double().cpu().numpy():
+        l = np.where(np.isnan(row[:E]), -np.inf, row[:E])
+        with np.errstate(all="ignore"):
+            if score == "softmax":
+                m = l.max()
+                s = np.zeros(E) if m == -np.inf else np.where(l == m, 1.0, np.exp(l - m))
+                s = s / s.sum() if s.sum() else s
+            else:
+                s = 0.5 * (1 + np.tanh(l / 2))
+                s = np.where(l < -30, np.exp(l), s)
+        if bias is None:
+            c, v = l.copy(), s if group_top == 2 else l
+        else:
+            b = bias.double().cpu().numpy()
+            c = v = s + np.where(np.isnan(b), -np.inf, b)
+        if groups > 1:
+            best = np.sort(v.reshape(groups, -1), 1)[:, ::-1][:, :group_top]
+            value = np.where((best == -np.inf).any(1), -np.inf, best.sum(1))
+            keep = np.argsort(-value, kind="stable")[:topk_groups]
+            out = np.repeat(~np.isin(np.arange(groups), keep), E // groups)
+        else:
+            out = np.zeros(E, bool)
+        order = np.lexsort((np.arange(E), -c, out))[:k]
+        w = s[order]
+        if norm:
+            w = w / w.sum() if w.sum() else w
+        idx.append(order)
+        wt.append(w * np.float64(np.float32(scale)))
+        sg.append(1 / (1 + np.exp(-row[E])) if gate else 1.0)
+    return np.array(idx), np.array(wt), np.array(sg)
+
+
+def check_route(logits, E, k, **kw):
+    got = [t.cpu().numpy() for t in _ops().moe_route_ex(logits, E, k, **kw)]
+    full = dict(score="softmax", bias=None, groups=1, topk_groups=1, group_top=1, norm=True, scale=1.0)
+    full.update(kw)
+    gate = full.pop("shared_gate", False)
+    idx, wt, sg = plain_route(logits, E, k, gate=gate, **full)
+    assert np.array_equal(got[0], idx)
+    # 64-bit values, rounded once; the 64-bit steps themselves are off by a few 2^-53
+    for g, w in ((got[1], wt), (got[2], sg)):
+        assert np.all(np.abs(g - w) <= 2.0 ** -24 * (1 + 1e-6) * np.abs(w) + 1e-44)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,E,k,groups,keep,top,bias", [
+    (1, 1, 1, 1, 1, 1, False), (5, 7, 7, 1, 1, 1, True), (3, 60, 4, 1, 1, 1, False), (65, 64, 6, 8, 3, 1, False),
+    (33, 100, 8, 10, 4, 2, True), (70, 128, 16, 2, 1, 2, False), (130, 160, 6, 8, 3, 1, True), (64, 256, 8, 8, 4, 2, True),
+    (1000, 256, 8, 8, 4, 2, True), (17, 96, 5, 3, 2, 2, True), (200, 512, 10, 1, 1, 1, False), (99, 512, 16, 64, 9, 2, True),
+    (31, 512, 8, 16, 16, 1, True), (40, 510, 12, 5, 3, 2, False), (2, 384, 9, 4, 1, 2, True), (77, 320, 8, 16, 3, 2, True),
+])
+def test_route(score, bf16, T, E, k, groups, keep, top, bias):
+    g = torch.Generator(device="cuda").manual_seed(T * E + k)
+    l = 1.5 * torch.randn((T, E + 1), device="cuda", generator=g)
+    b = 0.1 * torch.randn((E,), device="cuda", generator=g) if bias else None
+    l = l.to(torch.bfloat16) if bf16 else l
+    for norm, scale, gate in ((True, 1.0, False), (False, 2.5, True)):
+        check_route(l, E, k, score=score, bias=b, groups=groups, topk_groups=keep, group_top=top, norm=norm, scale=scale,
+                    shared_gate=gate)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("groups,keep,top", [(1, 1, 1), (8, 4, 1), (8, 4, 2), (5, 2, 2)])
+def test_route_edges(score, bias, groups, keep, top):
+    """Ties, masked experts, infinities and NaN, rows that a mask leaves empty, all in one batch."""
+    E, k = 160, 8
+    g = torch.Generator(device="cuda").manual_seed(7)
+    l = torch.randn((14, E), device="cuda", generator=g)
+    l[0] = 0.0
+    l[1] = -math.inf
+    l[2, 5:] = -math.inf
+    l[3] = torch.finfo(torch.float32).min
+    l[4, ::3] = torch.finfo(torch.float32).min
+    l[5, 17] = math.inf
+    l[6, 100:] = math.nan
+    l[7] = math.nan
+    l[8] = l[8].round()
+    l[9] = torch.where(l[9] > 0, 0.0, -0.0)
+    l[10] = 100 * l[10]
+    l[11, 50] = l[11, 60] = math.inf
+    l[12] = 30 + l[12] * 1e-6
+    b = None
+    if bias:
+        b = (0.1 * torch.randn((E,), device="cuda", generator=g)).round(decimals=1)
+        b[3] = -math.inf
+        b[4] = math.nan
+    check_route(l, E, k, score=score, bias=b, groups=groups, topk_groups=keep, group_top=top)
+
+
+def test_route_near_ties_are_decided_in_64_bits():
+    """Sigmoid scores and biases whose sums differ by less than a rounding of fp32."""
+    T, E = 256, 128
+    g = torch.Generator(device="cuda").manual_seed(3)
+    l = torch.randn((T, E), device="cuda", generator=g)
+    s = torch.sigmoid(l[0].double())
+    l[:] = l[0] + torch.randint(-2, 3, (T, E), device="cuda", generator=g) * 2.0 ** -23
+    check_route(l, E, 16, score="sigmoid", bias=(0.7 - s).float(), norm=True)
+
+
+def test_route_agrees_with_the_plain_softmax_routing():
+    ops = _ops()
+    l = torch.randn((300, 513), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    a = ops.moe_route(l, 512, 10, norm=True, shared_gate=True)
+    b = ops.moe_route_ex(l, 512, 10, shared_gate=True)
+    assert torch.equal(a[0], b[0])
+    # fp32 exponentials and sums of 512 terms against 64-bit ones
+    assert torch.allclose(a[1], b[1], rtol=2e-6, atol=0) and torch.allclose(a[2], b[2], rtol=1e-6, atol=0)
+
+
+def test_route_writes_only_its_rows():
+    ops = _ops()
+    big = torch.randn((9, 400), device="cuda")
+    l = big[:, 37:37 + 65]  # a stride and an alignment of their own
+    outs = [torch.full((12, 4), -7, dtype=torch.int32, device="cuda"), torch.full((12, 4), -7.0, device="cuda"),
+            torch.full((12,), -7.0, device="cuda")]
+    ops.moe_route_ex(l, 64, 4, score="sigmoid", shared_gate=True, outs=tuple(t[:9] for t in outs))
+    assert all(bool((t[9:] == -7).all()) for t in outs)
+    ref = plain_route(l, 64, 4, "sigmoid", None, 1, 1, 1, True, 1.0, True)
+    assert np.array_equal(outs[0][:9].cpu().numpy(), ref[0])
+
+
+# ---- sampling --------------------------------------------------------------------------------------------------------
+def plain_sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    """ifd_sample's rule, row by row in 64 bits."""
+    tokens, probs = [], []
+    at = lambda t, r, off: off if t is None else float(t[r])  # noqa: E731
+    u = u.cpu().numpy()
+    temperature, top_k, top_p, min_p = (None if t is None else t.cpu().numpy() for t in (temperature, top_k, top_p, min_p))
+    for r, l in enumerate(logits.double().cpu().numpy()):
+        l = np.where(np.isnan(l), -np.inf, l)
+        V, m = len(l), l.max()
+        tau = at(temperature, r, 1.0)
+        if m == -np.inf or not tau > 0:
+            tokens.append(-1 if m == -np.inf else int(l.argmax()))
+            probs.append(0.0 if m == -np.inf else 1.0)
+            continue
+        with np.errstate(all="ignore"):
+            w = np.where(l == m, 1.0, np.exp((l - m) / tau))
+        w[w <= 2.0 ** -45] = 0.0
+        order = np.argsort(-l, kind="stable")
+        k = int(at(top_k, r, 0))
+        n = k if 0 < k < V else V
+        p = at(top_p, r, 1.0)
+        if not p >= 1:
+            c = np.cumsum(w[order[:n]])
+            n = min(n, 1 + int(np.searchsorted(c, (p if p > 0 else 0.0) * c[-1])))
+        kept = order[:n]
+        mp = at(min_p, r, 0.0)
+        kept = np.sort(kept[w[kept] >= min(mp, 1.0)] if mp > 0 else kept)
+        c = np.cumsum(w[kept])
+        x = min(max(float(u[r]), 0.0) if u[r] == u[r] else 0.0, 1 - 2.0 ** -24)
+        t = kept[np.searchsorted(c, x * c[-1], side="right")]
+        tokens.append(int(t))
+        probs.append(w[t] / c[-1])
+    return np.array(tokens), np.array(probs)
+
+
+def check_sample(logits, u, **kw):
+    token, prob = (t.cpu().numpy() for t in _ops().sample(logits, u, **kw))
+    want, p = plain_sample(logits, u, **kw)
+    bad = np.flatnonzero(token != want)
+    assert not len(bad), (bad[:8], token[bad[:8]], want[bad[:8]])
+    # a rounding to fp32, and weights rounded to 2^-45 of the largest (their total is at least 1)
+    V = logits.shape[1]
+    assert np.all(np.abs(prob - p) <= 2.0 ** -24 * (1 + 1e-6) * p + 2.0 ** -44 * (1 + V * p))
+
+
+def _lm_logits(T, V, seed, bf16=False, std=2.2):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    l = std * torch.randn((T, V), device="cuda", generator=g)
+    n = min(V, 30)
+    l.scatter_(1, torch.randint(0, V, (T, n), device="cuda", generator=g),
+               6 + 6 * torch.rand((T, n), device="cuda", generator=g))
+    u = torch.rand((T,), device="cuda", generator=g)
+    return (l.to(torch.bfloat16) if bf16 else l), u, g
+
+
+def _col(T, values, dtype=torch.float32):
+    return torch.tensor([values[i % len(values)] for i in range(T)], dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,V", [(1, 1), (3, 2), (4, 63), (5, 1000), (2, 4096), (1, 50021), (17, 50021), (3, 151936),
+                                 (1, 248320), (40, 20000), (1, 1 << 19), (130, 3001)])
+@pytest.mark.parametrize("kind", ["none", "k", "p", "kp", "min", "all"])
+def test_sample(bf16, T, V, kind):
+    l, u, _ = _lm_logits(T, V, T + V, bf16)
+    kw = dict(temperature=_col(T, [1.0, 0.7, 0.1, 1.5, 0.0, 5.0]))
+    if kind in ("k", "kp", "all"):
+        kw["top_k"] = _col(T, [40, 1, 0, V, 1000, 5000, 7, -3], torch.int32)
+    if kind in ("p", "kp", "all"):
+        kw["top_p"] = _col(T, [0.9, 0.5, 1.0, 0.99, 1e-6, 0.999999, 0.0])
+    if kind in ("min", "all"):
+        kw["min_p"] = _col(T, [0.05, 0.0, 1e-4, 0.5, 1.0])
+    for i in range(2):
+        check_sample(l, u if i == 0 else 1 - u, **kw)
+
+
+def test_sample_sizes_are_all_alike_on_ties():
+    """Few distinct logits, so that every border falls among equal ones: the lower indices are kept."""
+    for V, levels in ((1000, 1), (1000, 3), (30001, 2), (151936, 1), (151936, 17), (248320, 5)):
+        T = 24
+        g = torch.Generator(device="cuda").manual_seed(V + levels)
+        l = torch.randint(0, levels, (T, V), device="cuda", generator=g).float() * 0.37 - 3
+        u = torch.rand((T,), device="cuda", generator=g)
+        for kw in (dict(top_p=_col(T, [0.5, 0.9, 0.123, 0.999])), dict(top_k=_col(T, [5, 100, 999, 4097], torch.int32)),
+                   dict(top_k=_col(T, [900, 333, 50], torch.int32), top_p=_col(T, [0.5, 0.8])), dict()):
+            check_sample(l, u, temperature=_col(T, [1.0, 0.3]), **kw)
+
+
+def test_sample_edges():
+    """Masks, infinities, NaN, empty rows, and random numbers at and past the ends."""
+    V = 5000
+    l, u, g = _lm_logits(24, V, 11)
+    l[0] = -math.inf
+    l[1] = math.nan
+    l[2, 1:] = -math.inf
+    l[3, :-1] = -math.inf
+    l[4] = torch.finfo(torch.float32).min
+    l[5, 10:] = torch.finfo(torch.float32).min
+    l[6, 77] = math.inf
+    l[7, 77] = l[7, 99] = math.inf
+    l[8, ::2] = math.nan
+    l[9, 4000:] = -math.inf
+    l[10] = 0.0
+    l[11] = torch.where(l[11] > 0, 0.0, -0.0)
+    l[12] = 1e30 * l[12]
+    l[13] = 1e-30 * l[13]
+    u[14:20] = torch.tensor([0.0, 1.0, 1 - 2.0 ** -24, 2.0, -1.0, math.nan], device="cuda")
+    T = len(l)
+    for kw in (dict(), dict(top_k=_col(T, [3], torch.int32)), dict(top_p=_col(T, [0.9])), dict(min_p=_col(T, [0.1])),
+               dict(top_k=_col(T, [100], torch.int32), top_p=_col(T, [0.7]), min_p=_col(T, [0.01])),
+               dict(top_p=_col(T, [math.nan, -1.0, 2.0])), dict(min_p=_col(T, [math.nan, -1.0, 2.0]))):
+        for tau in (None, [1.0], [0.0, -1.0, math.nan], [1e-3], [1e3], [1e-30]):
+            check_sample(l, u, temperature=None if tau is None else _col(T, tau), **kw)
+
+
+def test_sample_frequencies_follow_the_weights():
+    """Many random numbers on one row: each token's share is its weight (chi-square, fixed seed)."""
+    n, V = 20000, 50
+    g = torch.Generator(device="cuda").manual_seed(5)
+    l = torch.randn((1, V), device="cuda", generator=g)
+    token, prob = _ops().sample(l.expand(n, V).contiguous(), torch.rand((n,), device="cuda", generator=g))
+    p = torch.softmax(l[0].double(), 0).cpu().numpy()
+    seen = np.bincount(token.cpu().numpy(), minlength=V)
+    chi = float(((seen - n * p) ** 2 / (n * p)).sum())
+    assert chi < 49 + 6 * math.sqrt(2 * 49)  # six standard deviations of a chi-square with 49 degrees of freedom
+    assert np.allclose(prob.cpu().numpy(), p[token.cpu().numpy()], rtol=1e-6)
+
+
+def test_sample_strides_and_untouched_rows():
+    big = torch.randn((6, 3001), device="cuda").to(torch.bfloat16)
+    l = big[:, 3:3 + 2500]
+    u = torch.rand((6,), device="cuda")
+    token, prob = torch.full((9,), -7, dtype=torch.int32, device="cuda"), torch.full((9,), -7.0, device="cuda")
+    _ops().sample(l, u, top_p=_col(6, [0.8]), outs=(token[:6], prob[:6]))
+    assert bool((token[6:] == -7).all()) and bool((prob[6:] == -7).all())
+    assert np.array_equal(token[:6].cpu().numpy(), plain_sample(l, u, top_p=_col(6, [0.8]))[0])
+
+
+# ---- linears with an epilogue ------------------------------------------------------------------------------------------
+def _act64(y, act):
+    if act == "relu":
+        return torch.where(y < 0, torch.zeros_like(y), y)
+    if act == "silu":
+        return y / (1 + torch.exp(-y))
+    if act == "gelu":
+        return y * 0.5 * torch.special.erfc(-y / math.sqrt(2))
+    if act == "gelu_tanh":
+        return y / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)))
+    return y
+
+
+def _layer(N, K, bits, seed):
+    g, ops = _gu(), _ops()
+    codes, wq, s, b = gen.qlinear(N, K, seed=seed, bias="free") if bits == 4 else gen.qlinear8(N, K, seed=seed, bias="free")
+    W = (ops.pack_t64 if bits == 4 else ops.pack_t64x8)(g.qlinear(wq, s, b, bits=bits))
+    return W, torch.from_numpy(gen.dequant_f64(codes, s, b)).cuda()
+
+
+def _weights_as_used(w, M, N, K, bits):
+    """The weights in the arithmetic that the product runs at these sizes."""
+    from oracle import oracle as orc
+    from tests.test_gpu_t64 import _t64_arith
+    exact = M <= 16 and K % 128 == 0 if bits == 8 else _t64_arith(M, N, K) is orc.qmv
+    return w if exact else w.to(torch.bfloat16).double()
+
+
+def check_epi(M, N, K, bits, act, bias, res, fp32=False, inplace=False, seed=0, A=None, W=None):
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(seed + M + N)
+    layer, w = W or _layer(N, K, bits, seed + 1)
+    A = torch.randn((M, K), device="cuda", generator=g).to(torch.bfloat16) if A is None else A
+    b = torch.randn((N,), device="cuda", generator=g).to(torch.bfloat16) if bias else None
+    r = (2 * torch.randn((M, N), device="cuda", generator=g)).to(torch.bfloat16) if res else None
+    w = _weights_as_used(w, M, N, K, bits)
+    y = A.double() @ w.T.contiguous()
+    # the fp32 sum of K products (and the groups' own steps), through an activation of slope at most 1.13
+    tol = 1.13 * (K + 16) * 2.0 ** -24 * (A.double().abs() @ w.abs().T.contiguous())
+    y = y if b is None else y + b.double()
+    a = _act64(y, act)
+    # the activation in fp32: a few roundings of its value, and those of the exponent's argument
+    tol = tol + 2.0 ** -20 * (a.abs() + y.abs().clamp(max=8) * 2.0 ** -4 + 2.0 ** -20)
+    a = a if r is None else a + r.double()
+    C = r if inplace else None
+    out = (ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi)(A, layer, bias=b, act=act, residual=r, C=C, fp32=fp32)
+    assert out.dtype == (torch.float32 if fp32 else torch.bfloat16)
+    assert not inplace or out.data_ptr() == r.data_ptr()
+    err = (out.double() - a).abs() - HALF[out.dtype] * (a.abs() + tol) - tol
+    worst = int(err.argmax())
+    assert float(err.max()) <= 0, (worst // N, worst % N, float(out.flatten()[worst]), float(a.flatten()[worst]))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("M,N,K", [(1, 256, 512), (16, 1000, 1024), (17, 129, 256), (64, 512, 512), (100, 1024, 512),
+                                   (300, 768, 512)])
+def test_epilogue_activations(bits, act, M, N, K):
+    W = _layer(N, K, bits, 3)
+    for bias, res, fp32 in ((True, True, False), (False, False, True), (True, False, True), (False, True, False)):
+        check_epi(M, N, K, bits, act, bias, res, fp32=fp32, W=W)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 9, 16, 17, 32, 33, 64, 65, 96, 97, 128, 129, 161, 256, 333, 1000])
+@pytest.mark.parametrize("N,K", [(32, 256), (100, 256), (129, 512), (1, 256), (256, 1024), (1000, 768), (5120, 1024)])
+def test_epilogue_shapes(M, N, K):
+    check_epi(M, N, K, 4, "silu", True, True)
+
+
+@pytest.mark.parametrize("M", [1, 9, 16, 17, 33, 65, 129, 300])
+@pytest.mark.parametrize("N,K", [(32, 64), (100, 128), (129, 320), (1, 256), (1000, 768), (5120, 1024)])
+def test_epilogue_shapes_8bit(M, N, K):
+    check_epi(M, N, K, 8, "gelu", True, True)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 5120, 5120), (8, 5120, 17408), (16, 34816, 5120), (32, 34816, 5120), (128, 5120, 17408),
+                                   (777, 5120, 5120), (1300, 5120, 2048)])
+def test_epilogue_split_products(M, N, K, bits):
+    """Sizes at which K is split among blocks, so that the epilogue runs where the pieces are joined."""
+    W = _layer(N, K, bits, 9)
+    check_epi(M, N, K, bits, "none", True, True, inplace=True, W=W)
+    check_epi(M, N, K, bits, "gelu_tanh", True, False, W=W)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M", [5, 40, 100, 150, 700])
+def test_epilogue_without_any_step_is_the_plain_product(bits, M):
+    ops = _ops()
+    N, K = 640, 1024
+    layer, _ = _layer(N, K, bits, 4)
+    A = torch.randn((M, K), device="cuda").to(torch.bfloat16)
+    for mode in (0, 1, 2):
+        C = torch.randn((M, N), device="cuda").to(torch.bfloat16) if mode == 1 else None
+        D = C.clone() if mode == 1 else None
+        a = (ops.gemm_t64 if bits == 4 else ops.gemm_t64x8)(A, layer, C, mode=mode)
+        b = (ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi)(A, layer, residual=D, C=D, fp32=mode == 2)
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,N", [(3, 100), (20, 100), (100, 260), (140, 256), (200, 333)])
+def test_epilogue_strides(M, N, bits):
+    """Rows apart and off alignment in A, C and the residual; what lies between and behind the rows stays."""
+    ops = _ops()
+    K = 512
+    layer, w = _layer(N, K, bits, 5)
+    A = torch.randn((M, K + 24), device="cuda").to(torch.bfloat16)[:, 8:8 + K]
+    bias = torch.randn((N,), device="cuda").to(torch.bfloat16)
+    R = torch.randn((M, N + 13), device="cuda").to(torch.bfloat16)[:, 5:5 + N]
+    for dtype in (torch.bfloat16, torch.float32):
+        big = torch.full((M + 2, N + 7), 7.0, device="cuda", dtype=dtype)
+        out = big[1:M + 1, 3:3 + N]
+        (ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi)(A, layer, bias=bias, act="relu", residual=R, C=out)
+        ww = _weights_as_used(w, M, N, K, bits)
+        y = A.double() @ ww.T.contiguous()
+        ref = torch.relu(y + bias.double()) + R.double()
+        tol = (K + 16) * 2.0 ** -24 * (A.double().abs() @ ww.abs().T.contiguous()) + 2.0 ** -20
+        assert bool(((out.double() - ref).abs() <= HALF[dtype] * (ref.abs() + tol) + tol).all())
+        rest = big.clone()
+        rest[1:M + 1, 3:3 + N] = 7.0
+        assert bool((rest == 7.0).all())
+
+
+@pytest.mark.parametrize("M", [2, 24, 100, 140])
+def test_epilogue_infinities_and_nan(M):
+    """Infinities and NaN in the bias and the residual come out as the formula has them, and nowhere else."""
+    ops = _ops()
+    N, K = 256, 256
+    layer, w = _layer(N, K, 4, 6)
+    A = torch.randn((M, K), device="cuda").to(torch.bfloat16)
+    bias = torch.zeros((N,), device="cuda", dtype=torch.bfloat16)
+    bias[3], bias[5], bias[7] = math.inf, -math.inf, math.nan
+    R = torch.zeros((M, N), device="cuda", dtype=torch.bfloat16)
+    R[1, 10], R[1, 11], R[0, 12] = math.nan, math.inf, -math.inf
+    for act in ("none", "relu", "silu", "gelu", "gelu_tanh"):
+        out = ops.gemm_t64_epi(A, layer, bias=bias, act=act, residual=R).double()
+        ref = _act64(A.double() @ _weights_as_used(w, M, N, K, 4).T.contiguous() + bias.double(), act) + R.double()
+        assert torch.equal(out.isnan(), ref.isnan()), act
+        assert torch.equal(out == math.inf, ref == math.inf) and torch.equal(out == -math.inf, ref == -math.inf), act
