@@ -399,14 +399,9 @@ int check_epi(const void* A, int lda, const void* wt, int N, int K, const uint16
   }
   return IFD_OK;
 }
-// The product goes to the workspace in fp32, behind the GEMM's own: [gemm | y [M][N]].
-size_t epi_ws(size_t gemm, int M, int N) { return with_header(align_up(gemm, 256) + (size_t)M * N * sizeof(float)); }
 }  // namespace
 
-size_t ifd_gemm_t64_epi_workspace(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K % 256) return 0;
-  return epi_ws(M <= 16 ? qmv_t_workspace(M, N, K, 2) : gemm_t_workspace(M, N, K, 2), M, N);
-}
+size_t ifd_gemm_t64_epi_workspace(int M, int N, int K) { return K % 256 ? 0 : ifd_gemm_t64_workspace(M, N, K); }
 
 int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
                      const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace, size_t ws_bytes,
@@ -414,21 +409,14 @@ int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const
   IFD_CHECK(M >= 0 && N > 0 && K > 0 && K % 256 == 0, "bad shape M=%d N=%d K=%d (K multiple of 256)", M, N, K);
   IFD_TRY(check_epi(A, lda, wt, N, K, bias, act, res, ldr, C, ldc, M, out_f32, workspace));
   if (M == 0) return IFD_OK;
-  const size_t need = ifd_gemm_t64_epi_workspace(M, N, K);
-  if (!workspace || ws_bytes < need)
-    return fail(IFD_ERR_WORKSPACE, "gemm_t64_epi needs %zu bytes of workspace, got %zu", need, ws_bytes);
   const WsView w = ws_view(workspace, ws_bytes);
-  const size_t gemm = need - kWsHeader - (size_t)M * N * sizeof(float);
-  float* y = (float*)((char*)w.body + gemm);
-  IFD_TRY(M <= 16 ? launch_qmv_t((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.cnt, w.body, gemm, S(stream))
-                  : launch_gemm_t((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.body, gemm, S(stream)));
-  return launch_epi(y, M, N, Epi{bias, (const uint16_t*)res, ldr, act}, C, ldc, out_f32, S(stream));
+  const Epi e{bias, (const uint16_t*)res, ldr, act, out_f32};
+  if (M <= 16)
+    return launch_qmv_t((const uint16_t*)A, lda, wt, N, K, C, ldc, M, kModeEpi, w.cnt, w.body, w.bytes, S(stream), &e);
+  return launch_gemm_t((const uint16_t*)A, lda, wt, N, K, C, ldc, M, kModeEpi, w.body, w.bytes, S(stream), &e);
 }
 
-size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K % 64) return 0;
-  return epi_ws(t64x8_qmv(M, K) ? qmv_t_workspace(M, N, K, 2, 8) : gemm_sk8_workspace(M, N, K), M, N);
-}
+size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K) { return ifd_gemm_t64x8_workspace(M, N, K); }
 
 int ifd_gemm_t64x8_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
                        const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace,
@@ -436,15 +424,11 @@ int ifd_gemm_t64x8_epi(const void* A, int lda, const void* wt, int N, int K, con
   IFD_CHECK(M >= 0 && N > 0 && K > 0 && K % 64 == 0, "bad shape M=%d N=%d K=%d (K multiple of 64)", M, N, K);
   IFD_TRY(check_epi(A, lda, wt, N, K, bias, act, res, ldr, C, ldc, M, out_f32, workspace));
   if (M == 0) return IFD_OK;
-  const size_t need = ifd_gemm_t64x8_epi_workspace(M, N, K);
-  if (!workspace || ws_bytes < need)
-    return fail(IFD_ERR_WORKSPACE, "gemm_t64x8_epi needs %zu bytes of workspace, got %zu", need, ws_bytes);
   const WsView w = ws_view(workspace, ws_bytes);
-  const size_t gemm = need - kWsHeader - (size_t)M * N * sizeof(float);
-  float* y = (float*)((char*)w.body + gemm);
-  IFD_TRY(t64x8_qmv(M, K) ? launch_qmv_t8((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.cnt, w.body, gemm, S(stream))
-                          : launch_gemm_sk8((const uint16_t*)A, lda, wt, N, K, y, N, M, 2, w.body, gemm, S(stream)));
-  return launch_epi(y, M, N, Epi{bias, (const uint16_t*)res, ldr, act}, C, ldc, out_f32, S(stream));
+  const Epi e{bias, (const uint16_t*)res, ldr, act, out_f32};
+  if (t64x8_qmv(M, K))
+    return launch_qmv_t8((const uint16_t*)A, lda, wt, N, K, C, ldc, M, kModeEpi, w.cnt, w.body, w.bytes, S(stream), &e);
+  return launch_gemm_sk8((const uint16_t*)A, lda, wt, N, K, C, ldc, M, kModeEpi, w.body, w.bytes, S(stream), &e);
 }
 
 // ---- sampling --------------------------------------------------------------------------------------------------------

@@ -11,16 +11,78 @@ struct Epi {
   const uint16_t* res = nullptr;   // bf16 [M][ldr], or null; may be C itself
   int ldr = 0;
   int act = kActNone;
+  int f32 = 0;  // C is fp32, else bf16
 };
 
-__device__ __forceinline__ float epi_act(float v, int act) {
-  switch (act) {  // uniform over the launch
-    case kActRelu: return v < 0.f ? 0.f : v;
-    case kActSilu: return v / (1.f + expf(-v));
-    case kActGelu: return v * 0.5f * erfcf(v * -0.70710678118654752f);
-    case kActGeluTanh: return v / (1.f + expf(-1.5957691216057308f * (v + 0.044715f * v * v * v)));
-    default: return v;
+// 2^x and 1 / x to one unit in the last place by the hardware's estimates (results below 2^-126 are 0). Off the device
+// (the tests run some kernels' source on the host) the library's.
+#ifdef __HIP__
+__device__ __forceinline__ float epi_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float epi_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+#else
+inline float epi_exp2(float x) { return exp2f(x); }
+inline float epi_rcp(float x) { return 1.f / x; }
+#endif
+
+// The activations in as few instructions as fp32 takes (an epilogue of a GEMM whose waves stand alone on their SIMD pays
+// about 5 cycles for each): 5 for SILU, 7 for GELU_TANH, 15 for GELU. Infinities and NaN as the formulas have them.
+__device__ __forceinline__ float act_silu(float x) { return x * epi_rcp(1.f + epi_exp2(x * -1.44269504f)); }
+// x / (1 + exp(-2 sqrt(2 / pi) (x + 0.044715 x^3)))
+__device__ __forceinline__ float act_gelu_tanh(float x) {
+  return x * epi_rcp(1.f + epi_exp2(x * __builtin_fmaf(x * x, -0.102943240f, -2.30220819f)));
+}
+// x Phi(x): with t = 1 / (1 + p z), z = |x| / sqrt 2, Phi(-|x|) = exp(-z^2) t (a1 + t (a2 + ..)) / 2 to 7.5e-8
+// (Abramowitz and Stegun 7.1.26)
+__device__ __forceinline__ float act_gelu(float x) {
+  const float t = epi_rcp(__builtin_fmaf(fabsf(x), 0.3275911f * 0.707106781f, 1.f));
+  float q = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  q = __builtin_fmaf(q, t, 0.5f * 1.421413741f);
+  q = __builtin_fmaf(q, t, 0.5f * -0.284496736f);
+  q = __builtin_fmaf(q, t, 0.5f * 0.254829592f);
+  q = q * t * epi_exp2(x * x * (-0.5f * 1.44269504f));
+  return x * (x < 0.f ? q : 1.f - q);
+}
+
+// act is uniform over a launch: one branch for all N values. CLASS: the activations that are compiled in (kEpiAny, or one
+// of the others, by epi_class): a kernel that unrolls its epilogue over many registers takes one class.
+enum EpiClass { kEpiLinear, kEpiSigmoid, kEpiErf, kEpiAny };
+__host__ __device__ inline int epi_class(int act) {
+  return act <= kActRelu ? kEpiLinear : act == kActGelu ? kEpiErf : kEpiSigmoid;
+}
+template <int N, int CLASS = kEpiAny>
+__device__ __forceinline__ void epi_act(float (&v)[N], int act) {
+  constexpr bool any = CLASS == kEpiAny;
+  if ((any || CLASS == kEpiLinear) && act == kActNone) return;
+  if ((any || CLASS == kEpiLinear) && act == kActRelu) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+  } else if ((any || CLASS == kEpiSigmoid) && act == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = act_silu(v[i]);
+  } else if ((any || CLASS == kEpiErf) && act == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = act_gelu(v[i]);
+  } else if (any || CLASS == kEpiSigmoid) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = act_gelu_tanh(v[i]);
   }
+}
+
+// N values of one row from column col on (o: the first's place in C), of which n lie in the row.
+template <int N>
+__device__ __forceinline__ void epi_store(const Epi& e, void* C, size_t o, int row, int col, int n, float (&v)[N]) {
+  float b[N], r[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    b[i] = e.bias && i < n ? bf2f(e.bias[col + i]) : 0.f;
+    r[i] = e.res && i < n ? bf2f(e.res[(size_t)row * e.ldr + col + i]) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] += b[i];
+  epi_act(v, e.act);
+#pragma unroll
+  for (int i = 0; i < N; i++)
+    if (i < n) store_mode(C, o + i, e.res ? v[i] + r[i] : v[i], e.f32 ? 2 : 0);
 }
 
 }  // namespace ifd

@@ -1,28 +1,26 @@
-// The epilogue of a linear as a pass of its own over the fp32 product in the workspace.
+// The sum of a K split's partials with the linear's epilogue, where the GEMM's own blocks do not join them: rows whose
+// length is no multiple of four in the decode GEMV.
 #include "epi.h"
 #include "host.h"
 #include "kernels.h"
 
 namespace ifd {
 
-__global__ __launch_bounds__(256) void k_epi(const float* __restrict__ y, int M, int N, Epi e, void* C, int ldc,
-                                             int out_f32) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (size_t)M * N) return;
+__global__ __launch_bounds__(256) void k_splitk_epi(const float* __restrict__ part, int S, int M, int N, Epi e, void* C,
+                                                    int ldc) {
+  const size_t mn = (size_t)M * N, i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= mn) return;
   const int m = (int)(i / N), n = (int)(i % N);
-  float v = y[i];
-  if (e.bias) v += bf2f(e.bias[n]);
-  v = epi_act(v, e.act);
-  if (e.res) v += bf2f(e.res[(size_t)m * e.ldr + n]);
-  store_mode(C, (size_t)m * ldc + n, v, out_f32 ? 2 : 0);
+  float v[1] = {0.f};
+  for (int z = 0; z < S; z++) v[0] += part[z * mn + i];
+  epi_store(e, C, (size_t)m * ldc + n, m, n, 1, v);
 }
 
-int launch_epi(const float* y, int M, int N, const Epi& e, void* C, int ldc, int out_f32, hipStream_t st) {
+int launch_splitk_epi(const float* part, int S, int M, int N, const Epi& e, void* C, int ldc, hipStream_t st) {
   const size_t n = (size_t)M * N;
   if (n == 0) return IFD_OK;
-  if ((n + 255) / 256 > 0x7fffffffu) return fail(IFD_ERR_UNSUPPORTED, "epilogue: %d x %d is too large", M, N);
-  hipLaunchKernelGGL(k_epi, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, y, M, N, e, C, ldc, out_f32);
-  return check_launch("epilogue");
+  hipLaunchKernelGGL(k_splitk_epi, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, S, M, N, e, C, ldc);
+  return check_launch("split-K epilogue");
 }
 
 }  // namespace ifd

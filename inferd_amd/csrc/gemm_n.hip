@@ -40,6 +40,7 @@
 
 #include "common.h"
 #include "dma.h"
+#include "epi.h"
 #include "host.h"
 #include "kernels.h"
 #include "share.h"
@@ -70,6 +71,7 @@ struct GemmNArgs {
   int half;           // bands per half of the columns (N % 128 == 0), or 0: a tile is 4 neighbouring bands
   int full;           // tiles 0 .. full - 1 are summed whole, block b taking b, b + gridDim.x, ..
   int rem, nsk;       // the rem other tiles' rounds are shared evenly among blocks 0 .. nsk - 1 (rem < nsk)
+  Epi e;              // MODE kModeEpi
 };
 
 // physical band of wave w's band nb of tile t (may lie past the last one when half == 0)
@@ -100,6 +102,21 @@ __device__ __forceinline__ void n_emit(const GemmNArgs& p, int t, int w, int r0,
 #pragma unroll
       for (int e = 0; e < 4; e++)
         old[e] = bf2f(((const uint16_t*)p.C)[(size_t)min(r0 + e, p.M - 1) * p.ldc + min(col, p.N - 1)]);
+    if constexpr (MODE == kModeEpi) {
+      const float bias = p.e.bias ? bf2f(p.e.bias[min(col, p.N - 1)]) : 0.f;
+      if (p.e.res)
+#pragma unroll
+        for (int e = 0; e < 4; e++) old[e] = bf2f(p.e.res[(size_t)min(r0 + e, p.M - 1) * p.e.ldr + min(col, p.N - 1)]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] += bias;
+      epi_act(v, p.e.act);
+      if (col < p.N)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (r0 + e < p.M)
+            store_mode(p.C, (size_t)(r0 + e) * p.ldc + col, p.e.res ? v[e] + old[e] : v[e], p.e.f32 ? 2 : 0);
+      continue;
+    }
     if (col < p.N)
 #pragma unroll
       for (int e = 0; e < 4; e++)
@@ -490,18 +507,21 @@ static int launch_n_cfg(const GemmNArgs& a, hipStream_t st) {
     case kModeSwiglu:
       if constexpr (FORM != 2) return launch_n_mode<MT, NKQ, FORM, NS, kModeSwiglu>(a, st);
       return fail(IFD_ERR_UNSUPPORTED, "gemm_n: no SwiGLU on int8 rows");
+    case kModeEpi:
+      if constexpr (FORM != 2) return launch_n_mode<MT, NKQ, FORM, NS, kModeEpi>(a, st);
+      return fail(IFD_ERR_UNSUPPORTED, "gemm_n: no epilogue on int8 rows");
     default: return launch_n_mode<MT, NKQ, FORM, NS, 0>(a, st);
   }
 }
 
 int launch_gemm_n(const uint16_t* A, int lda, const float* sxT, int Mp, const void* wt, int N, int K, void* C, int ldc,
-                  int M, int mode, int form, void* ws, size_t ws_bytes, hipStream_t st) {
+                  int M, int mode, int form, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
   if (M == 0) return IFD_OK;
   if ((size_t)M * lda * 2 >= ((size_t)1 << 31) || (size_t)(K / kGroup) * Mp * 4 >= ((size_t)1 << 31))
     return fail(IFD_ERR_UNSUPPORTED, "gemm_n: operands past 2 GiB");
   const NPlan pl = n_plan(M, N, K, form, ws ? ws_bytes : 0);
   GemmNArgs a{A, lda, (const uint8_t*)wt, (uint32_t)t64_bytes(N, K), N, K, C, ldc, M, mode, sxT, Mp, pl.tiles_m, (float*)ws,
-              N % 128 == 0 ? N / 64 : 0, pl.full, pl.rem, pl.nsk};
+              N % 128 == 0 ? N / 64 : 0, pl.full, pl.rem, pl.nsk, epi ? *epi : Epi{}};
   if (form == 2) return pl.MT == 1 ? launch_n_cfg<1, 4, 2, 3>(a, st) : launch_n_cfg<2, 4, 2, 3>(a, st);
   if (pl.MT == 1) return form ? launch_n_cfg<1, 4, 1, 3>(a, st) : launch_n_cfg<1, 4, 0, 3>(a, st);
   if (pl.MT == 2) return form ? launch_n_cfg<2, 4, 1, 3>(a, st) : launch_n_cfg<2, 4, 0, 3>(a, st);

@@ -29,6 +29,7 @@
 
 #include "common.h"
 #include "dma.h"
+#include "epi.h"
 #include "host.h"
 #include "kernels.h"
 #include "t64.h"
@@ -74,6 +75,7 @@ struct GemmSkArgs {
   const float* rs;
   int rs_stride;
   int sparse;  // more blocks than units: some runs are empty
+  Epi e;       // EPI: what is stored
 };
 
 // the block whose run holds unit u
@@ -109,7 +111,7 @@ __device__ __forceinline__ void sk_static_for(F&& f) {
 // register set is a compile-time constant; a run enters it at its phase (Duff's device). A step issues about 220
 // instructions for its 8 MT MFMAs, which a single wave per SIMD issues one every ~4 cycles: the stream's bookkeeping
 // is a few scalar adds and one countdown per step.
-template <int MT>
+template <int MT, bool EPI>
 __device__ __forceinline__ void sk_body(const GemmSkArgs& p, uint8_t* lds, const int wave, const int b) {
   constexpr int BM = 32 * MT, R = sk_ring(MT), A_BYTES = sk_abytes(MT), STAGE = sk_stage(MT);
   constexpr int CODES = kT64x8Codes, TILEB = kT64x8Tile;
@@ -373,6 +375,11 @@ __device__ __forceinline__ void sk_body(const GemmSkArgs& p, uint8_t* lds, const
       if (grow >= p.M || gcol >= p.N) continue;
       const float* sv = stg + row * kSkRow + c4;
       const size_t o = (size_t)grow * p.ldc + gcol;
+      if constexpr (EPI) {
+        float v[4] = {sv[0], sv[1], sv[2], sv[3]};
+        epi_store(p.e, p.C, o, grow, gcol, p.N - gcol, v);
+        continue;
+      }
       if (gcol + 4 <= p.N && (o & 3) == 0 && p.mode != 1) {
         if (p.mode == 2) *(float4*)((float*)p.C + o) = *(const float4*)sv;
         else *(u32x2*)((uint16_t*)p.C + o) = u32x2{pack_bf2(sv[0], sv[1]), pack_bf2(sv[2], sv[3])};
@@ -396,13 +403,13 @@ __device__ __forceinline__ void sk_body(const GemmSkArgs& p, uint8_t* lds, const
   write_slot(2 * b + (two ? 1 : 0));  // a piece of a cut tile: k_sk_fixup sums the pieces
 }
 
-template <int MT>
+template <int MT, bool EPI = false>
 __global__ __launch_bounds__(kSkThreads, 1) void k_gemm_sk(GemmSkArgs p) {
   static_assert(sk_lds(MT) + 64 <= kSkLds, "LDS plan");
   extern __shared__ __align__(16) uint8_t lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = xcd_remap(blockIdx.x, p.nblk);
-  sk_body<MT>(p, lds, wave, b);
+  sk_body<MT, EPI>(p, lds, wave, b);
 }
 
 // Sum of a cut tile's pieces (partial slots, in unit order) and its store. Block (tile, w, a), wave q: the float4
@@ -410,7 +417,7 @@ __global__ __launch_bounds__(kSkThreads, 1) void k_gemm_sk(GemmSkArgs p) {
 // stored by the GEMM kernel. blockIdx.x is the
 // tile's index among the stream-K tiles (units [tile G, tile G + G) of their U = ntiles G).
 constexpr int kFixBatch = 8;
-template <int MT>
+template <int MT, bool EPI = false>
 __global__ __launch_bounds__(256) void k_sk_fixup(GemmSkArgs p) {
   constexpr int BM = 32 * MT, NE = MT * 16;
   const int tile = blockIdx.x, w = blockIdx.y, a = blockIdx.z, q = threadIdx.x >> 6;
@@ -454,6 +461,14 @@ __global__ __launch_bounds__(256) void k_sk_fixup(GemmSkArgs p) {
   }
   const int col = (8 * tn + w) * 32 + j;
   if (col >= p.N) return;
+  if constexpr (EPI) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float y[1] = {vv[e]};
+      if (row0 + e < p.M) epi_store(p.e, p.C, (size_t)(row0 + e) * p.ldc + col, row0 + e, col, 1, y);
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (row0 + e < p.M) store_mode(p.C, (size_t)(row0 + e) * p.ldc + col, vv[e], p.mode);
@@ -498,18 +513,18 @@ size_t gemm_sk_workspace(int M, int N, int K, int mode) {
 
 size_t gemm_sk8_workspace(int M, int N, int K) { return sk_part_bytes(gemm_sk_plan(M, N, K, 8)); }
 
-template <int MT>
+template <int MT, bool EPI>
 static int launch_sk_cfg(const GemmSkArgs& a, bool fixup, hipStream_t st) {
   constexpr size_t lds = sk_lds(MT);
   static bool attr = false;
   if (!attr) {
-    (void)hipFuncSetAttribute((const void*)k_gemm_sk<MT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    (void)hipFuncSetAttribute((const void*)k_gemm_sk<MT, EPI>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     attr = true;
   }
-  hipLaunchKernelGGL((k_gemm_sk<MT>), dim3(a.nblk), dim3(kSkThreads), lds, st, a);
+  hipLaunchKernelGGL((k_gemm_sk<MT, EPI>), dim3(a.nblk), dim3(kSkThreads), lds, st, a);
   IFD_TRY(check_launch("gemm_sk"));
   if (!fixup) return IFD_OK;
-  hipLaunchKernelGGL(k_sk_fixup<MT>, dim3(a.ntiles, 8, MT), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_sk_fixup<MT, EPI>), dim3(a.ntiles, 8, MT), dim3(256), 0, st, a);
   return check_launch("gemm_sk fixup");
 }
 
@@ -525,7 +540,7 @@ int launch_sk_fixup_rows(const float* part, int tiles_m, int tiles_n, int tile0,
 }
 
 static int launch_sk(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                     void* ws, size_t ws_bytes, hipStream_t st) {
+                     void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
   const SkPlan pl = gemm_sk_plan(M, N, K, 8);
   const size_t need = sk_part_bytes(pl), wbytes = t64x8_bytes(N, K);
   if (need > ws_bytes || !ws)
@@ -541,18 +556,22 @@ static int launch_sk(const uint16_t* A, int lda, const void* wt, int N, int K, v
   for (long t = 0; t < tiles && !fixup; t++)
     fixup = sk_block_of(t * pl.G + pl.G - 1, pl.nblk, U) != sk_block_of(t * pl.G, pl.nblk, U);
   GemmSkArgs a{A, lda, (const uint8_t*)wt, (uint32_t)wbytes, N, K, C, ldc, M, mode, (float*)ws, (uint32_t)need,
-               pl.tiles_m, pl.tiles_n, pl.G, pl.nblk, 0, (int)tiles, nullptr, 0, 0};
-  if (pl.MT == 1) return launch_sk_cfg<1>(a, fixup, st);
-  if (pl.MT == 2) return launch_sk_cfg<2>(a, fixup, st);
-  return launch_sk_cfg<4>(a, fixup, st);
+               pl.tiles_m, pl.tiles_n, pl.G, pl.nblk, 0, (int)tiles, nullptr, 0, 0, epi ? *epi : Epi{}};
+  if (mode == kModeEpi) {
+    if (pl.MT == 1) return launch_sk_cfg<1, true>(a, fixup, st);
+    return pl.MT == 2 ? launch_sk_cfg<2, true>(a, fixup, st) : launch_sk_cfg<4, true>(a, fixup, st);
+  }
+  if (pl.MT == 1) return launch_sk_cfg<1, false>(a, fixup, st);
+  if (pl.MT == 2) return launch_sk_cfg<2, false>(a, fixup, st);
+  return launch_sk_cfg<4, false>(a, fixup, st);
 }
 
 int launch_gemm_sk8(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                    void* ws, size_t ws_bytes, hipStream_t st) {
+                    void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
   if (M == 0) return IFD_OK;
   if (K % kGroup || mode == kModeSwiglu)
     return fail(IFD_ERR_UNSUPPORTED, "gemm_sk8: N=%d K=%d mode=%d", N, K, mode);
-  return launch_sk(A, lda, wt, N, K, C, ldc, M, mode, ws, ws_bytes, st);
+  return launch_sk(A, lda, wt, N, K, C, ldc, M, mode, ws, ws_bytes, st, epi);
 }
 
 }  // namespace ifd

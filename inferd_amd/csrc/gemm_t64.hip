@@ -408,7 +408,7 @@ int launch_gemm_t_a8(const uint16_t* Ab, const float* sxT, int Mp, const void* w
 }
 
 int launch_gemm_t(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  void* ws, size_t ws_bytes, hipStream_t st) {
+                  void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
   if (M == 0) return IFD_OK;
   if (K % 128) return fail(IFD_ERR_ARG, "T64 GEMM needs K %% 128 == 0 (K=%d)", K);
   if (tiles256_fill(M, N) && t64_bytes(N, K) >= ((size_t)1 << 31))
@@ -424,8 +424,8 @@ int launch_gemm_t(const uint16_t* A, int lda, const void* wt, int N, int K, void
       return fail(IFD_ERR_WORKSPACE, "gemm_t64 needs %zu bytes of workspace, got %zu", gemm_t_workspace(M, N, K, mode),
                   ws_bytes);
     const bool affine = gemm_n_affine(M, N, K, mode);
-    if (w) return launch_gemm_w(A, lda, wt, N, K, C, ldc, M, mode, ws, ws_bytes, st);
-    if (n) return launch_gemm_n(A, lda, nullptr, 0, wt, N, K, C, ldc, M, mode, affine, ws, ws_bytes, st);
+    if (w) return launch_gemm_w(A, lda, wt, N, K, C, ldc, M, mode, ws, ws_bytes, st, epi);
+    if (n) return launch_gemm_n(A, lda, nullptr, 0, wt, N, K, C, ldc, M, mode, affine, ws, ws_bytes, st, epi);
     // [the product's pieces | the product], in the SwiGLU's own arithmetic: the stream-K rule never took these widths, so
     // up to 64 rows it is the affine one
     const size_t product = (size_t)M * N * sizeof(uint16_t);
@@ -435,6 +435,8 @@ int launch_gemm_t(const uint16_t* A, int lda, const void* wt, int N, int K, void
                                        : launch_gemm_n(A, lda, nullptr, 0, wt, N, K, gu, N, M, 0, affine, ws, pieces, st));
     return launch_silu_mul(gu, N, (uint16_t*)C, ldc, N / 2, M, st);
   }
+  if (mode == kModeEpi)
+    return fail(IFD_ERR_UNSUPPORTED, "gemm_t64: weights or activations past 2 GiB (M=%d N=%d K=%d) have no epilogue", M, N, K);
   const GtPlan pl = gemm_t_plan(M, N, K);
   const size_t need = epilogue_ws_bytes(pl.S, M, N, mode);
   if (need > ws_bytes || (need && !ws))

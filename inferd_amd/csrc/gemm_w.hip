@@ -38,6 +38,7 @@
 
 #include "common.h"
 #include "dma.h"
+#include "epi.h"
 #include "host.h"
 #include "kernels.h"
 #include "share.h"
@@ -67,6 +68,7 @@ struct GemmWArgs {
   int half;           // bands per half of the columns (N % 256 == 0), or 0: a tile is 8 neighbouring bands
   int full;           // tiles 0 .. full - 1 are summed whole, block b taking b, b + gridDim.x, ..
   int rem, nsk;       // the rem other tiles' groups are shared evenly among blocks 0 .. nsk - 1 (rem < nsk)
+  Epi e;              // kWEpi, kWEpiScalar
 };
 
 // tile order: bands of kWBand M tiles, M fastest, so that neighbouring blocks (one XCD) share weight tiles in L2
@@ -103,7 +105,19 @@ __device__ __forceinline__ void w_swap32(uint32_t& lo, uint32_t& hi) {
 // one value at a time by the runtime mode, with the MFMA's operands exchanged so that a lane holds one column of 16 rows
 // and a store's lanes neighbouring columns. A template parameter: with all of them in one kernel the epilogue's registers
 // spill the sums.
-enum WStore { kWBf16 = 0, kWAdd = 1, kWF32 = 2, kWSwiglu = kModeSwiglu, kWScalar = 4 };
+// The linear's epilogue (p.e) has a form of either kind: kWEpi + class of the activation writes bf16 (the bias 8-byte
+// aligned, and the residual with its rows), kWEpiScalar either type. With every activation in one kernel the epilogues of
+// 192 rows and more spill sums (17 to 104 registers), and past 160 rows the scalar one is too long to be unrolled: it takes
+// tiles of 128 and 160.
+enum WStore { kWBf16 = 0, kWAdd = 1, kWF32 = 2, kWSwiglu = kModeSwiglu, kWScalar = 4, kWEpiScalar = 5, kWEpi = 6 };
+__host__ __device__ constexpr bool w_scalar(int ST) { return ST == kWScalar || ST == kWEpiScalar; }
+__host__ __device__ constexpr bool w_epi(int ST) { return ST >= kWEpiScalar; }
+__host__ __device__ constexpr int w_class(int ST) { return ST >= kWEpi ? ST - kWEpi : (int)kEpiAny; }
+// whether values are added to the sums (old): mode 1's, or the epilogue's residual
+template <int ST>
+__device__ __forceinline__ bool w_adds(const GemmWArgs& p) {
+  return w_epi(ST) ? p.e.res != nullptr : ST == kWAdd || (ST == kWScalar && p.mode == 1);
+}
 
 // Sixteen bf16 values of one row in a band (this lane: columns 8 q + 4 h + e, value v[4 q + e]) to `row` (the band's
 // first column, of n more columns), 16 bytes per store; lanes that are not live only take part in the swaps.
@@ -127,29 +141,53 @@ struct WOld {
 };
 template <int ST>
 __device__ __forceinline__ void w_load_old(const GemmWArgs& p, int row, int tn, int w, int j, int h, WOld& old) {
+  const uint16_t* const src = w_epi(ST) ? p.e.res : (const uint16_t*)p.C;
+  const int ld = w_epi(ST) ? p.e.ldr : p.ldc;
 #pragma unroll
   for (int nb = 0; nb < 2; nb++) {
     const int col = w_band(p, tn, w, nb) * 32;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      if constexpr (ST == kWAdd) {
-        const size_t o = (size_t)min(row, p.M - 1) * p.ldc + min(col + 8 * q, p.N - 8) + 4 * h;
-        old.c[nb][q] = *(const u32x2*)((const uint16_t*)p.C + o);
+      if constexpr (!w_scalar(ST)) {
+        const size_t o = (size_t)min(row, p.M - 1) * ld + min(col + 8 * q, p.N - 8) + 4 * h;
+        old.c[nb][q] = *(const u32x2*)(src + o);
       } else {
         uint32_t v[4];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          v[e] = ((const uint16_t*)p.C)[(size_t)min(row - j + 8 * q + 4 * h + e, p.M - 1) * p.ldc + min(col + j, p.N - 1)];
+          v[e] = src[(size_t)min(row - j + 8 * q + 4 * h + e, p.M - 1) * ld + min(col + j, p.N - 1)];
         old.c[nb][q] = u32x2{v[0] | v[1] << 16, v[2] | v[3] << 16};
       }
     }
   }
 }
 
-// The sums of wave w's two bands in one row tile of column tile tn, stored (old: the values that mode 1 adds to).
+// The bias of a wave's two bands: with kWEpi this lane's 16 columns of each as bf16 pairs (past N those of the last columns,
+// which nothing uses), kWEpiScalar that of its column.
+struct WBias {
+  u32x2 c[2][4];
+};
+template <int ST>
+__device__ __forceinline__ void w_load_bias(const GemmWArgs& p, int tn, int w, int j, int h, WBias& bias) {
+#pragma unroll
+  for (int nb = 0; nb < 2; nb++) {
+    const int col = w_band(p, tn, w, nb) * 32;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      if (w_scalar(ST) && q > 0) continue;
+      bias.c[nb][q] = u32x2{0u, 0u};
+      if (!p.e.bias) continue;
+      if constexpr (!w_scalar(ST)) bias.c[nb][q] = *(const u32x2*)(p.e.bias + min(col + 8 * q, p.N - 8) + 4 * h);
+      else bias.c[nb][q][0] = p.e.bias[min(col + j, p.N - 1)];
+    }
+  }
+}
+
+// The sums of wave w's two bands in one row tile of column tile tn, stored (old: the values that mode 1 or the epilogue
+// adds).
 template <int ST>
 __device__ __forceinline__ void w_emit(const GemmWArgs& p, int row, int tn, int w, int j, int h, const f32x16& x0,
-                                       const f32x16& x1, const WOld& old) {
+                                       const f32x16& x1, const WOld& old, const WBias& bias) {
   const bool live = row < p.M;
   float v[2][16];
 #pragma unroll
@@ -166,14 +204,21 @@ __device__ __forceinline__ void w_emit(const GemmWArgs& p, int row, int tn, int 
     const int col = w_band(p, tn, w, nb) * 32, n = p.N - col;
     if (n <= 0) continue;  // wave-uniform
     const size_t o = (size_t)row * p.ldc + col;
-    if (ST == kWAdd || (ST == kWScalar && p.mode == 1))
+    if constexpr (w_epi(ST)) {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        v[nb][e] += bf2f((uint16_t)(w_scalar(ST) ? bias.c[nb][0][0] : bias.c[nb][e / 4][e % 4 / 2] >> (16 * (e % 2))));
+      epi_act<16, w_class(ST)>(v[nb], p.e.act);
+    }
+    if (w_adds<ST>(p))
 #pragma unroll
       for (int e = 0; e < 16; e++) v[nb][e] += bf2f((uint16_t)(old.c[nb][e / 4][e % 4 / 2] >> (16 * (e % 2))));
-    if constexpr (ST == kWScalar) {
+    if constexpr (w_scalar(ST)) {
 #pragma unroll
       for (int e = 0; e < 16; e++) {
         const int r = row - j + 8 * (e / 4) + 4 * h + e % 4;
-        if (j < n && r < p.M) store_mode(p.C, (size_t)r * p.ldc + col + j, v[nb][e], p.mode & 2);
+        if (j < n && r < p.M)
+          store_mode(p.C, (size_t)r * p.ldc + col + j, v[nb][e], w_epi(ST) ? (p.e.f32 ? 2 : 0) : p.mode & 2);
       }
     } else if constexpr (ST == kWF32) {
 #pragma unroll
@@ -353,7 +398,7 @@ __global__ __launch_bounds__(256, 1) void k_gemm_w(GemmWArgs p) {
         }
 #pragma unroll
         for (int nb = 0; nb < 2; nb++)
-          acc[nb][g] = ST == kWScalar ? mfma_bf16(af[t & 1][g], bf[nb][t], acc[nb][g])
+          acc[nb][g] = w_scalar(ST) ? mfma_bf16(af[t & 1][g], bf[nb][t], acc[nb][g])
                                       : mfma_bf16(bf[nb][t], af[t & 1][g], acc[nb][g]);
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
@@ -399,11 +444,13 @@ __global__ __launch_bounds__(256, 1) void k_gemm_w(GemmWArgs p) {
       int tm, tn;
       w_tile(t, p.tiles_m, p.tiles_n, tm, tn);
       // the residual rows of up to four row tiles are requested together: their latency is paid per group
-      constexpr int GA = ST == kWAdd ? 4 : ST == kWScalar ? 2 : 1;
+      constexpr int GA = ST == kWAdd ? 4 : w_epi(ST) ? (MT == 8 ? 1 : 2) : ST == kWScalar ? 2 : 1;
       WOld old[GA];
+      WBias bias;
+      if constexpr (w_epi(ST)) w_load_bias<ST>(p, tn, wave, j, h, bias);
 #pragma unroll
       for (int a = 0; a < MT; a++) {
-        if (a % GA == 0 && (ST == kWAdd || (ST == kWScalar && p.mode == 1))) {
+        if (a % GA == 0 && w_adds<ST>(p)) {
 #pragma unroll
           for (int i = 0; i < GA; i++)
             if (a + i < MT) w_load_old<ST>(p, tm * BM + 32 * (a + i) + j, tn, wave, j, h, old[i]);
@@ -414,7 +461,7 @@ __global__ __launch_bounds__(256, 1) void k_gemm_w(GemmWArgs p) {
         for (int nb = 0; nb < 2; nb++)
 #pragma unroll
           for (int e = 0; e < 16; e++) asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x[nb][e]) : "a"(acc[nb][a][e]));
-        w_emit<ST>(p, tm * BM + 32 * a + j, tn, wave, j, h, x[0], x[1], old[a % GA]);
+        w_emit<ST>(p, tm * BM + 32 * a + j, tn, wave, j, h, x[0], x[1], old[a % GA], bias);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -440,7 +487,9 @@ __global__ __launch_bounds__(256) void k_gemm_w_fixup(GemmWArgs p) {
       (const float4*)p.part + (size_t)share_piece(b0, tile, p.rem, p.nsk) * 8 * MT * 4 * 64 + lane;
   f32x16 x[2] = {zero16(), zero16()};
   WOld old;
-  if (p.mode == 1) w_load_old<ST>(p, tm * 32 * MT + 32 * a + j, tn, wave, j, h, old);
+  WBias bias;
+  if constexpr (w_epi(ST)) w_load_bias<ST>(p, tn, wave, j, h, bias);
+  if (w_epi(ST) ? p.e.res != nullptr : p.mode == 1) w_load_old<ST>(p, tm * 32 * MT + 32 * a + j, tn, wave, j, h, old);
 #pragma unroll 2
   for (int z = 0; z <= b1 - b0; z++) {
     float4 v[2][4];
@@ -456,7 +505,7 @@ __global__ __launch_bounds__(256) void k_gemm_w_fixup(GemmWArgs p) {
         x[nb][4 * q + 2] += v[nb][q].z, x[nb][4 * q + 3] += v[nb][q].w;
       }
   }
-  w_emit<ST>(p, tm * 32 * MT + 32 * a + j, tn, wave, j, h, x[0], x[1], old);
+  w_emit<ST>(p, tm * 32 * MT + 32 * a + j, tn, wave, j, h, x[0], x[1], old, bias);
 }
 
 // ---- host side
@@ -495,9 +544,9 @@ static WPlan w_plan_mt(int MT, int M, int N, int K, size_t part_bytes) {
 }
 // The row-tile height with the least estimated time: it fits M (a 777-row prompt is five tiles of 160 rows rather than
 // four of 256) and the CUs' rounds.
-static WPlan w_plan(int M, int N, int K, size_t part_bytes) {
-  WPlan best = w_plan_mt(8, M, N, K, part_bytes);
-  for (int MT = 7; MT >= 4; MT--) {
+static WPlan w_plan(int M, int N, int K, size_t part_bytes, int most = 8) {
+  WPlan best = w_plan_mt(most, M, N, K, part_bytes);
+  for (int MT = most - 1; MT >= 4; MT--) {
     const WPlan pl = w_plan_mt(MT, M, N, K, part_bytes);
     if (pl.ns < best.ns) best = pl;
   }
@@ -529,8 +578,21 @@ static int launch_w_cfg(const GemmWArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((k_gemm_w_fixup<MT, ST>), dim3(a.rem, MT), dim3(256), 0, st, a);
   return check_launch("gemm_w fixup");
 }
+static bool w_epi_vec(const void* C, int ldc, int N, const Epi& e) {
+  return aligned(C, 16) && ldc % 8 == 0 && N % 16 == 0 && !e.f32 && aligned(e.bias, 8) && aligned(e.res, 8) &&
+         e.ldr % 4 == 0;
+}
 template <int MT>
 static int launch_w_st(const GemmWArgs& a, hipStream_t st) {
+  if (a.mode == kModeEpi) {
+    if constexpr (MT <= 5)
+      if (!w_epi_vec(a.C, a.ldc, a.N, a.e)) return launch_w_cfg<MT, kWEpiScalar>(a, st);
+    switch (epi_class(a.e.act)) {
+      case kEpiSigmoid: return launch_w_cfg<MT, kWEpi + kEpiSigmoid>(a, st);
+      case kEpiErf: return launch_w_cfg<MT, kWEpi + kEpiErf>(a, st);
+      default: return launch_w_cfg<MT, kWEpi + kEpiLinear>(a, st);
+    }
+  }
   const bool vec = aligned(a.C, 16) && a.ldc % (a.mode == 2 ? 4 : 8) == 0 && a.N % 16 == 0;
   if (!vec) return launch_w_cfg<MT, kWScalar>(a, st);
   switch (a.mode) {
@@ -542,12 +604,13 @@ static int launch_w_st(const GemmWArgs& a, hipStream_t st) {
 }
 
 int launch_gemm_w(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  void* ws, size_t ws_bytes, hipStream_t st) {
+                  void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
   if (M == 0) return IFD_OK;
   if ((size_t)M * lda * 2 >= ((size_t)1 << 31)) return fail(IFD_ERR_UNSUPPORTED, "gemm_w: operands past 2 GiB");
-  const WPlan pl = w_plan(M, N, K, ws ? std::min(ws_bytes, kWPartMax) : 0);
+  const WPlan pl = w_plan(M, N, K, ws ? std::min(ws_bytes, kWPartMax) : 0,
+                          mode == kModeEpi && !w_epi_vec(C, ldc, N, *epi) ? 5 : 8);
   GemmWArgs a{A, lda, (const uint8_t*)wt, (uint32_t)t64_bytes(N, K), N, K, C, ldc, M, mode, (float*)ws, pl.tiles_m,
-              pl.tiles_n, N % 256 == 0 ? N / 64 : 0, pl.full, pl.rem, pl.nsk};
+              pl.tiles_n, N % 256 == 0 ? N / 64 : 0, pl.full, pl.rem, pl.nsk, epi ? *epi : Epi{}};
   switch (pl.MT) {
     case 4: return launch_w_st<4>(a, st);
     case 5: return launch_w_st<5>(a, st);

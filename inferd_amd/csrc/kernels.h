@@ -56,6 +56,9 @@ int launch_probe_mfma(int int8, int iters, int blocks, float* out, hipStream_t s
 // [gate (N/2) | up (N/2)] and C receives the SwiGLU h [M][N/2] (ldc = its row stride), bit-identical to a mode-0 GEMM
 // followed by silu_mul.
 constexpr int kModeSwiglu = 3;
+// Another: C receives what the launcher's Epi says (act(y + bias) + residual, bf16 or fp32), epi.h.
+constexpr int kModeEpi = 4;
+struct Epi;
 // Split-K reduction: C (mode) = sum over S partials [S][M][N] fp32, in split order.
 int launch_splitk_reduce(const float* part, int S, int M, int N, void* C, int ldc, int mode, hipStream_t st);
 // Workspace of a GEMM epilogue with S K-splits: the fp32 partials, or for the SwiGLU mode without a split the bf16
@@ -77,16 +80,16 @@ size_t gemm_t_least_workspace(int M, int N, int K, int mode);
 bool gemm_w_applies(int M, int N, int K, int mode);
 size_t gemm_w_workspace(int M, int N, int K);
 int launch_gemm_w(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  void* ws, size_t ws_bytes, hipStream_t st);
+                  void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 // GEMM on T64 weights for 16 < M <= 128 (gemm_n.hip), modes 0-2 and SwiGLU. form: 0 bf16-dequantized weights, 1 the
 // decode GEMV's arithmetic (up to 64 rows), 2 the W4A8 of gemm_t_a8 below (A its bf16 integers, sxT their scales).
 bool gemm_n_applies(int M, int N, int K, int mode);
 bool gemm_n_a8_applies(int M, int N, int K);
 size_t gemm_n_workspace(int M, int N, int K, int form);
 int launch_gemm_n(const uint16_t* A, int lda, const float* sxT, int Mp, const void* wt, int N, int K, void* C, int ldc,
-                  int M, int mode, int form, void* ws, size_t ws_bytes, hipStream_t st);
+                  int M, int mode, int form, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 int launch_gemm_t(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  void* ws, size_t ws_bytes, hipStream_t st);
+                  void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 // The stream-K plan (gemm_sk.hip) of a 4-bit shape: whether it has tiles for a third of the CUs (or one 128-row tile),
 // and its workspace, which such calls report at least and are served with.
 bool gemm_sk_applies(int M, int N, int K, int mode);
@@ -102,11 +105,11 @@ int launch_w4a8_t(const int8_t* U, const float* XS, const void* wt, int N, int K
 // The decode GEMV on T64x8 weights (M <= 16, K % 128 == 0; the qmv8 arithmetic s sum q x + b sum x); its workspace
 // is qmv_t_workspace(M, N, K, mode, 8).
 int launch_qmv_t8(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st);
+                  unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 // Stream-K GEMM (gemm_sk.hip) on T64x8 weights (8-bit codes, dequantized to bf16(s q + b)); any M >= 1.
 size_t gemm_sk8_workspace(int M, int N, int K);
 int launch_gemm_sk8(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                    void* ws, size_t ws_bytes, hipStream_t st);
+                    void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 // T64x8 (t64.h): the repack of an MLX 8-bit linear, and W8A8 on it with per-token int8 activations.
 int launch_pack_t64x8(const uint32_t* wq, const uint16_t* s, const uint16_t* b, int N, int K, int ldk, uint32_t xr,
                       void* out, hipStream_t st);
@@ -115,7 +118,7 @@ int launch_w8a8_t(const int8_t* U, const float* XS, const void* wt, int N, int K
                   void* ws, size_t ws_bytes, hipStream_t st);
 // cnt: kWsCounters zeroed counters (the workspace header) for the in-kernel split-K fixup; null -> a reduction kernel
 int launch_qmv_t(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                 unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st);
+                 unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi = nullptr);
 // n linears sharing A and K in one decode-GEMV launch (ifd_gemm_t64_multi)
 size_t qmv_t_multi_workspace(int M, int n, const int* Ns, int K);
 int launch_qmv_t_multi(const uint16_t* A, int lda, int n, const void* const* wts, const int* Ns, int K,
@@ -133,9 +136,8 @@ size_t gemm_t_a8_least_workspace(int M, int N, int K, int mode);
 int launch_gemm_t_a8(const uint16_t* Ab, const float* sxT, int Mp, const void* wt, int N, int K, void* C, int ldc,
                      int M, int mode, void* ws, size_t ws_bytes, hipStream_t st);
 
-// The epilogue of a linear, act(y + bias) + residual (epi.h), as a pass over its fp32 product y [M][N].
-struct Epi;
-int launch_epi(const float* y, int M, int N, const Epi& e, void* C, int ldc, int out_f32, hipStream_t st);
+// The sum of a K split's partials with the epilogue of a linear (epi.hip).
+int launch_splitk_epi(const float* part, int S, int M, int N, const Epi& e, void* C, int ldc, hipStream_t st);
 
 // Sampling (sample.hip): logits [T][ld] of V <= 1 << 19 columns; temperature, top_k, top_p, min_p and prob may be null.
 size_t sample_workspace(int T, int V);

@@ -793,7 +793,7 @@ static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream
   const dim3 block(256), grid(quads, a.T), some(std::min(quads, std::max(1, 1024 / a.T)), a.T);
   hipLaunchKernelGGL(k_sample_max<BF16>, grid, block, 0, st, a, ws);
   if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some, block, 0, st, a, ws);
-  if (a.T) hipLaunchKernelGGL(k_sample_collect<BF16>, some, block, 0, st, a, ws);
+  hipLaunchKernelGGL(k_sample_collect<BF16>, some, block, 0, st, a, ws);
   hipLaunchKernelGGL(k_sample_draw<BF16>, dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
   return check_launch("sample");
 }

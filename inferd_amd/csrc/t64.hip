@@ -5,6 +5,7 @@
 // s * sum q x + b * sum x in fp32, here with the products on bf16 MFMA (codes enter as exact bf16 (128 + q)) and the
 // group epilogue s * P + (b - 128 s) * X in fp32.
 #include "common.h"
+#include "epi.h"
 #include "host.h"
 #include "kernels.h"
 #include "t64.h"
@@ -83,6 +84,7 @@ struct QmvTArgs {
   int gps;
   const float* XS;  // A8: the rows' (sx, sx sum xq) per 64-group [M][K / 64][2] (A holds xq as bf16 integers)
   QmvTMulti mt;     // MULTI only
+  Epi e;            // EPI only
 };
 
 constexpr int kTB = 2;     // groups per pipeline block
@@ -105,7 +107,8 @@ __device__ __forceinline__ u32x4 t64_bf16_off128(uint32_t w) {
 // A8: the reference's W4A8 GEMM with per-(row, 64-group) int8 activations (w4a8.metal:24-98): A holds xq as exact
 // bf16 integers, so P and the group sums X are exact integers, and per group acc += sx (s P + (b - 128 s) X), the
 // row's group scale sx staged beside X.
-template <int RACT, int BITS, bool A8 = false, bool MULTI = false>
+// EPI: the sums are stored through the linear's epilogue (mode kModeEpi).
+template <int RACT, int BITS, bool A8 = false, bool MULTI = false, bool EPI = false>
 __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
   constexpr int NH = BITS / 4, TILEB = BITS == 8 ? kT64x8Tile : kT64Tile, CODES = BITS == 8 ? kT64x8Codes : kT64Codes;
   extern __shared__ __align__(16) uint16_t lds[];
@@ -244,7 +247,13 @@ __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
 #pragma unroll
     for (int r = 0; r < RACT; r++) {
       const int row = 8 * (r / 4) + 4 * h + (r % 4);
-      if (row < M) store_mode(Cl, (size_t)row * ldcl + col, acc[r], p.mode);
+      if (row >= M) continue;
+      if constexpr (EPI) {
+        float v[1] = {acc[r]};
+        epi_store(p.e, Cl, (size_t)row * ldcl + col, row, col, 1, v);
+      } else {
+        store_mode(Cl, (size_t)row * ldcl + col, acc[r], p.mode);
+      }
     }
     return;
   }
@@ -304,6 +313,11 @@ __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
       if (cl >= Nl) continue;
       const float4 v = sum4((size_t)row * p.N + c);
       const size_t o = (size_t)row * ldcl + cl;
+      if constexpr (EPI) {  // N % 4 == 0
+        float x[4] = {v.x, v.y, v.z, v.w};
+        epi_store(p.e, Cl, o, row, cl, 4, x);
+        continue;
+      }
       // a linear of the multi-linear launch may end inside the quad (its N need not be a multiple of 4)
       store_mode(Cl, o, v.x, p.mode);
       if (cl + 1 < Nl) store_mode(Cl, o + 1, v.y, p.mode);
@@ -357,7 +371,7 @@ size_t qmv_t_workspace(int M, int N, int K, int mode, int bits) {
 template <int BITS, bool A8 = false>
 static int launch_qmv_t_bits(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M,
                              int mode, unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st,
-                             const float* XS = nullptr) {
+                             const float* XS = nullptr, const Epi* epi = nullptr) {
   if (M == 0) return IFD_OK;
   if (M > 16) return fail(IFD_ERR_UNSUPPORTED, "T64 decode kernel takes M <= 16");
   if (K % (kGroup * kTB)) return fail(IFD_ERR_ARG, "T64 decode needs K %% %d == 0 (K=%d)", kGroup * kTB, K);
@@ -383,12 +397,21 @@ static int launch_qmv_t_bits(const uint16_t* A, int lda, const void* wt, int N, 
              fix && mode == kModeSwiglu ? (t64_bands(N) + 3) / 4 / 2 : 0,
              pl.gps,
              XS,
-             {}};
+             {},
+             epi ? *epi : Epi{}};
   const int Kz = pl.gps * kGroup;
   const size_t lds =
       ((size_t)M * (Kz + 8) * 2 + 15) / 16 * 16 + (size_t)pl.gps * 16 * sizeof(float) * (A8 ? 2 : 1);
   if (lds > 64 * 1024) return fail(IFD_ERR_UNSUPPORTED, "qmv_t64: %zu bytes of LDS needed", lds);
   dim3 grid((t64_bands(N) + 3) / 4, pl.S), block(256);
+  if constexpr (!A8) {
+    if (mode == kModeEpi) {
+      if (M <= 8) hipLaunchKernelGGL((k_qmv_t<4, BITS, false, false, true>), grid, block, lds, st, p);
+      else hipLaunchKernelGGL((k_qmv_t<8, BITS, false, false, true>), grid, block, lds, st, p);
+      IFD_TRY(check_launch("qmv_t64"));
+      return fix || pl.S == 1 ? IFD_OK : launch_splitk_epi((const float*)ws, pl.S, M, N, p.e, C, ldc, st);
+    }
+  }
   if (M <= 8) hipLaunchKernelGGL((k_qmv_t<4, BITS, A8>), grid, block, lds, st, p);
   else hipLaunchKernelGGL((k_qmv_t<8, BITS, A8>), grid, block, lds, st, p);
   IFD_TRY(check_launch("qmv_t64"));
@@ -428,7 +451,7 @@ int launch_qmv_t_multi(const uint16_t* A, int lda, int n, const void* const* wts
   if (pl.S > 1 && !(cnt && qmv_t_fixup(Ntot, mode, pl.S)))
     return fail(IFD_ERR_WORKSPACE, "qmv_t64 multi: a split launch needs the workspace's counter header");
   QmvTArgs p{A, lda, nullptr, Ntot, K, nullptr, 0, M, mode, (float*)ws, (uint32_t)(pl.S > 1 ? need : 0),
-             pl.S > 1 ? cnt : nullptr, 0, pl.gps, nullptr, mt};
+             pl.S > 1 ? cnt : nullptr, 0, pl.gps, nullptr, mt, Epi{}};
   const size_t lds = ((size_t)M * (pl.gps * kGroup + 8) * 2 + 15) / 16 * 16 + (size_t)pl.gps * 16 * sizeof(float);
   if (lds > 64 * 1024) return fail(IFD_ERR_UNSUPPORTED, "qmv_t64 multi: %zu bytes of LDS needed", lds);
   dim3 grid(bands / 4, pl.S), block(256);
@@ -438,13 +461,13 @@ int launch_qmv_t_multi(const uint16_t* A, int lda, int n, const void* const* wts
 }
 
 int launch_qmv_t(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                 unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st) {
-  return launch_qmv_t_bits<4>(A, lda, wt, N, K, C, ldc, M, mode, cnt, ws, ws_bytes, st);
+                 unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
+  return launch_qmv_t_bits<4>(A, lda, wt, N, K, C, ldc, M, mode, cnt, ws, ws_bytes, st, nullptr, epi);
 }
 
 int launch_qmv_t8(const uint16_t* A, int lda, const void* wt, int N, int K, void* C, int ldc, int M, int mode,
-                  unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st) {
-  return launch_qmv_t_bits<8>(A, lda, wt, N, K, C, ldc, M, mode, cnt, ws, ws_bytes, st);
+                  unsigned* cnt, void* ws, size_t ws_bytes, hipStream_t st, const Epi* epi) {
+  return launch_qmv_t_bits<8>(A, lda, wt, N, K, C, ldc, M, mode, cnt, ws, ws_bytes, st, nullptr, epi);
 }
 
 // The W4A8 form of the decode GEMV (per-group int8 activations): Ab = xq as bf16 integers [M][K], XS their

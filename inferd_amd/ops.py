@@ -10,6 +10,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import ctypes
+import functools
 
 import torch
 
@@ -24,7 +25,8 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (its handle alone: a Stream object costs 2.7 us per call)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 _ws_cache: dict = {}
@@ -41,34 +43,38 @@ def workspace(nbytes: int, device) -> torch.Tensor:
     return buf
 
 
-def _workspace_here(nbytes: int, device) -> torch.Tensor:
-    """A zeroed uint8 workspace for one call on the current stream: cached per device and stream, and a fresh one inside
-    a graph capture, so that calls on two streams, or two captured graphs, never share one."""
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, *sizes: int) -> int:
+    return getattr(lib(), query)(*sizes)
+
+
+def _workspace_here(nbytes: int, device, stream: int):
+    """The address of a zeroed workspace for one call on the current stream, and the tensor that holds it: cached per device
+    and stream, and a fresh one inside a graph capture, so that calls on two streams, or two captured graphs, never share
+    one."""
+    if nbytes == 0:
+        return None, None
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    key = (str(device), _stream())
-    buf = _ws_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
-        buf = _ws_cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return buf
+        buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    else:
+        key = (device.index, stream)
+        buf = _ws_cache.get(key)
+        if buf is None or buf.numel() < nbytes:
+            buf = _ws_cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return buf.data_ptr(), buf
 
 
-def _want(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _on_device(device, *tensors) -> None:
-    """Every tensor on `device`, which is the current one (the calls go to its current stream)."""
-    _want(device.type == "cuda" and device.index == torch.cuda.current_device(),
-          f"tensors on {device}, which is not the current device")
-    _want(all(t is None or t.device == device for t in tensors), "tensors on different devices")
-
-
-def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, name: str) -> None:
-    """None, or a tensor of this shape and type with adjacent values in a row."""
-    _want(t is None or (t.shape == shape and t.dtype == dtype), f"{name}: {shape} {dtype} wanted")
-    _want(t is None or t.shape[-1] == 1 or t.stride(-1) == 1, f"{name}: the values of a row must be adjacent")
+def _check_tensors(device, **tensors) -> None:
+    """Each argument is (tensor or None, shape, dtype): of that shape and type, its rows' values adjacent, on `device`, which
+    is the current one (the calls go to its current stream)."""
+    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on {device}, which is not the current device")
+    for name, (t, shape, dtype) in tensors.items():
+        if t is None:
+            continue
+        if t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and shape[-1] > 1):
+            raise ValueError(f"{name}: {tuple(shape)} {dtype} on {device} with adjacent values wanted, got "
+                             f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
 
 
 @dataclass
@@ -235,24 +241,22 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
 def _gemm_epi(name: str, A, W, bias, act, residual, C, fp32) -> torch.Tensor:
-    _want(A.dim() == 2 and A.dtype == torch.bfloat16 and A.shape[1] == W.K, f"A: bf16 [M, {W.K}] wanted")
-    M, N = A.shape[0], W.N
-    _on_device(A.device, W.wt, bias, residual, C)
-    _rows(A, (M, W.K), torch.bfloat16, "A")
-    _want(act in ACTS, f"act={act!r} must be one of {sorted(ACTS)}")
-    _rows(bias, (N,), torch.bfloat16, "bias")
-    _rows(residual, (M, N), torch.bfloat16, "residual")
+    if A.dim() != 2 or act not in ACTS:
+        raise ValueError(f"A: a matrix wanted, act={act!r}: one of {sorted(ACTS)}")
+    (M, K), N, dev, bf16 = A.shape, W.N, A.device, torch.bfloat16
     if C is None:
-        C = torch.empty((M, N), dtype=torch.float32 if fp32 else torch.bfloat16, device=A.device)
-    out = torch.float32 if C.dtype == torch.float32 else torch.bfloat16
-    _rows(C, (M, N), out, "C")
-    step = lambda t: t.stride(0) if M > 1 else t.shape[1]  # noqa: E731
-    L = lib()
-    need = getattr(L, name + "_workspace")(M, N, W.K)
-    ws = _workspace_here(need, A.device) if need else None
-    check(getattr(L, name)(_p(A), step(A), _p(W.wt), N, W.K, _p(bias), ACTS[act], _p(residual),
-                           0 if residual is None else step(residual), _p(C), step(C), M, int(out == torch.float32), _p(ws),
-                           need, _stream()))
+        C = torch.empty((M, N), dtype=torch.float32 if fp32 else bf16, device=dev)
+    f32 = C.dtype == torch.float32
+    _check_tensors(dev, A=(A, (M, W.K), bf16), bias=(bias, (N,), bf16), residual=(residual, (M, N), bf16),
+                   C=(C, (M, N), C.dtype if f32 else bf16), weights=(W.wt, (W.wt.numel(),), torch.uint8))
+    need = _workspace_bytes(name + "_workspace", M, N, K)
+    stream = _stream()
+    ws, _keep = _workspace_here(need, dev, stream)
+    lda, ldc, ldr = A.stride(0), C.stride(0), 0 if residual is None else residual.stride(0)
+    if M == 1:  # the stride of a single row says nothing
+        lda, ldc, ldr = K, N, N
+    check(getattr(lib(), name)(_p(A), lda, _p(W.wt), N, K, _p(bias), ACTS[act], _p(residual), ldr, _p(C), ldc, M, f32, ws,
+                               need, stream))
     return C
 
 
@@ -282,25 +286,20 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
 
     temperature, top_p, min_p fp32 [T] and top_k int32 [T] hold a value per row; None is off for all rows
     (temperature 0: greedy; top_k 0, top_p 1, min_p 0: off for that row). See ifd_sample for the rule."""
-    _want(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16), "logits: fp32 or bf16 [T, V] wanted")
-    T, V = logits.shape
-    _rows(logits, (T, V), logits.dtype, "logits")
-    for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
-                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                           ("min_p", min_p, torch.float32)):
-        _rows(t, (T,), dtype, name)
-    if outs is None:
-        outs = (torch.empty((T,), dtype=torch.int32, device=logits.device),
-                torch.empty((T,), dtype=torch.float32, device=logits.device))
-    token, prob = outs
-    _rows(token, (T,), torch.int32, "token")
-    _rows(prob, (T,), torch.float32, "prob")
-    _on_device(logits.device, u, temperature, top_k, top_p, min_p, token, prob)
-    need = lib().ifd_sample_workspace(T, V)
-    ws = _workspace_here(need, logits.device) if need else None
-    check(lib().ifd_sample(_p(logits), int(logits.dtype == torch.bfloat16), T, V, logits.stride(0) if T > 1 else V,
-                           _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(token), _p(prob), _p(ws), need,
-                           _stream()))
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"logits: a matrix of fp32 or bf16 wanted, got {tuple(logits.shape)} {logits.dtype}")
+    (T, V), dev, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
+    token, prob = outs if outs is not None else (torch.empty((T,), dtype=i32, device=dev),
+                                                 torch.empty((T,), dtype=f32, device=dev))
+    row = (T,)
+    _check_tensors(dev, logits=(logits, (T, V), logits.dtype), u=(u, row, f32), temperature=(temperature, row, f32),
+                   top_k=(top_k, row, i32), top_p=(top_p, row, f32), min_p=(min_p, row, f32), token=(token, row, i32),
+                   prob=(prob, row, f32))
+    need = _workspace_bytes("ifd_sample_workspace", T, V)
+    stream = _stream()
+    ws, _keep = _workspace_here(need, dev, stream)
+    check(lib().ifd_sample(_p(logits), logits.dtype == torch.bfloat16, T, V, logits.stride(0) if T > 1 else V,
+                           _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(token), _p(prob), ws, need, stream))
     return token, prob
 
 
@@ -444,25 +443,21 @@ def moe_route_ex(logits: torch.Tensor, E: int, k: int, score: str = "softmax", b
     topk_groups best stay, weights renormalised (norm) and scaled; see ifd_moe_route_ex for the rule. logits [T, >= E (+ 1
     with shared_gate)] fp32 or bf16. Returns (idx int32 [T, k], wt fp32 [T, k], sg fp32 [T]), as moe_route, written to
     `outs` when given."""
-    _want(logits.dim() == 2 and logits.dtype in (torch.float32, torch.bfloat16), "logits: fp32 or bf16 [T, E] wanted")
-    _want(score in SCORES, f"score={score!r} must be one of {sorted(SCORES)}")
-    T, width = logits.shape
-    _want(width >= E + (1 if shared_gate else 0), f"logits: {width} columns for E={E} (+ shared gate)")
-    _rows(logits, (T, width), logits.dtype, "logits")
-    _rows(bias, (E,), torch.float32, "bias")
-    dev = logits.device
-    if outs is None:
-        outs = (torch.empty((T, k), dtype=torch.int32, device=dev), torch.empty((T, k), dtype=torch.float32, device=dev),
-                torch.empty((T,), dtype=torch.float32, device=dev))
-    idx, wt, sg = outs
-    _want(idx.shape == wt.shape == (T, k) and sg.shape == (T,) and idx.dtype == torch.int32
-          and wt.dtype == sg.dtype == torch.float32 and all(t.is_contiguous() for t in outs),
-          f"outs: contiguous int32 [{T}, {k}], fp32 [{T}, {k}] and fp32 [{T}] wanted")
-    _on_device(dev, bias, idx, wt, sg)
-    check(lib().ifd_moe_route_ex(_p(logits), int(logits.dtype == torch.bfloat16), T, E, k,
-                                 logits.stride(0) if T > 1 else width, SCORES[score], _p(bias), groups,
-                                 topk_groups, group_top, int(norm), float(scale), int(shared_gate), _p(idx), _p(wt),
-                                 _p(sg), _stream()))
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or score not in SCORES:
+        raise ValueError(f"logits: a matrix of fp32 or bf16 wanted, score={score!r}: one of {sorted(SCORES)}")
+    (T, width), dev, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
+    if width < E + (1 if shared_gate else 0):
+        raise ValueError(f"logits: {width} columns for E={E} (+ shared gate)")
+    idx, wt, sg = outs if outs is not None else (torch.empty((T, k), dtype=i32, device=dev),
+                                                 torch.empty((T, k), dtype=f32, device=dev),
+                                                 torch.empty((T,), dtype=f32, device=dev))
+    _check_tensors(dev, logits=(logits, (T, width), logits.dtype), bias=(bias, (E,), f32), idx=(idx, (T, k), i32),
+                   wt=(wt, (T, k), f32), sg=(sg, (T,), f32))
+    if not (idx.is_contiguous() and wt.is_contiguous()):
+        raise ValueError("idx and wt must be contiguous")
+    check(lib().ifd_moe_route_ex(_p(logits), logits.dtype == torch.bfloat16, T, E, k, logits.stride(0) if T > 1 else width,
+                                 SCORES[score], _p(bias), groups, topk_groups, group_top, norm, scale, shared_gate, _p(idx),
+                                 _p(wt), _p(sg), _stream()))
     return idx, wt, sg
 
 
