@@ -26,6 +26,31 @@ __device__ __forceinline__ double exp_neg(double x) {
   return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
+// 2^y for y <= 0 as a whole number of 2^-44 (NaN and y < -64: 0), from 2^y to 4e-14: the nearest whole number n of y (the low
+// bits of y + 44 + 1.5 2^52) and a polynomial of degree 9 on [-1/2, 1/2] that takes 2^r - 1 over r at the Chebyshev points;
+// n + 44 is added to the exponent, and the sum with 2^52 has the result in its low bits. Conversions and ldexp run at a quarter
+// of the rate of these. 2^0 is 2^44 exactly.
+__device__ __forceinline__ uint64_t exp2_fixed44(double y) {
+  constexpr double kRound = 0x1.8p52 + 44;
+  y = fmax(y, -64.0);
+  const double m = y + kRound, r = y - (m - kRound);
+  double p = 1.0203121063391729e-07;
+  p = __builtin_fma(p, r, 1.3255224878668817e-06);
+  p = __builtin_fma(p, r, 1.525268684626772e-05);
+  p = __builtin_fma(p, r, 0.00015403455852453838);
+  p = __builtin_fma(p, r, 0.0013333558179043112);
+  p = __builtin_fma(p, r, 0.009618129159402558);
+  p = __builtin_fma(p, r, 0.055504108664760424);
+  p = __builtin_fma(p, r, 0.2402265069581299);
+  p = __builtin_fma(p, r, 0.6931471805599453);
+  p = __builtin_fma(p, r, 1.0);
+  u32x2 q = __builtin_bit_cast(u32x2, p);
+  q[1] += __builtin_bit_cast(u32x2, m)[0] << 20;
+  q = __builtin_bit_cast(u32x2, __builtin_bit_cast(double, q) + 0x1p52);
+  q[1] &= 0xfffffu;
+  return __builtin_bit_cast(uint64_t, q);
+}
+
 // 1 / d for 1 <= d <= 1e300: the reciprocal estimate and two Newton steps.
 __device__ __forceinline__ double rcp64(double d) {
   double r = __builtin_amdgcn_rcp(d);

@@ -30,9 +30,13 @@ struct SampleArgs {
   float* prob;  // or null
 };
 
+// w 2^44 of a logit of a row with a maximum above -infinity; rt = log2(e) / temperature
+__device__ __forceinline__ uint64_t weight(float l, float mx, double rt) {
+  return l == mx ? 1ull << 44 : exp2_fixed44(((double)l - (double)mx) * rt);
+}
 struct RowPar {
-  double rt;      // 1 / temperature
-  double min_p;
+  double rt;      // log2(e) / temperature
+  uint64_t min_w;  // min_p
   double top_p;
   int k;          // V: off
   bool greedy;
@@ -41,12 +45,12 @@ __device__ __forceinline__ RowPar row_par(const SampleArgs& p, int t) {
   RowPar r;
   const float tau = p.temperature ? p.temperature[t] : 1.f;
   r.greedy = !(tau > 0.f);
-  r.rt = r.greedy ? 1.0 : 1.0 / (double)tau;
+  r.rt = 1.4426950408889634074 / (r.greedy ? 1.0 : (double)tau);
   r.k = p.top_k ? p.top_k[t] : 0;
   if (r.k <= 0 || r.k > p.V) r.k = p.V;
   const float tp = p.top_p ? p.top_p[t] : 1.f, mp = p.min_p ? p.min_p[t] : 0.f;
   r.top_p = tp < 1.f ? fmax((double)tp, 0.0) : tp >= 1.f ? 1.0 : 0.0;
-  r.min_p = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
+  r.min_w = mp > 0.f ? (uint64_t)__builtin_rint(fmin((double)mp, 1.0) * 0x1p44) : 0;
   return r;
 }
 // a row's random number, inside [0, 1)
@@ -59,21 +63,15 @@ __device__ __forceinline__ float load_logit(const SampleArgs& p, int t, int i) {
   const size_t o = (size_t)t * p.ld + i;
   return order_value(BF16 ? bf2f(((const uint16_t*)p.logits)[o]) : ((const float*)p.logits)[o]);
 }
-// w of a logit of a row with a maximum above -infinity
-__device__ __forceinline__ double weight(float l, float mx, double rt) {
-  return l == mx ? 1.0 : exp_neg(((double)l - (double)mx) * rt);
-}
-__device__ __forceinline__ uint64_t fixed(double w) { return (uint64_t)__builtin_rint(w * 0x1p44); }
-
 // ---- one block per row ---------------------------------------------------------------------------------------------
-constexpr int kRowThreads = 1024, kRowBins = 2048;
+constexpr int kRowThreads = 512, kRowBins = 2048;
 struct RowLds {
   uint64_t w[kRowBins];
   uint32_t n[kRowBins];
   uint64_t wsum[64];
   uint32_t nsum[64];
-  uint64_t wpart[16];
-  uint32_t npart[16];
+  uint64_t wpart[kRowThreads / 64];
+  uint32_t npart[kRowThreads / 64];
   uint32_t key, ties;
   uint64_t total;
   int at;
@@ -128,7 +126,7 @@ __device__ Border row_border(RowLds& s, const SampleArgs& p, int t, float mx, do
       if (!by_count && key == in.key) continue;  // its `ties` ones are added below
       atomicAdd(&s.n[b], 1u);
       if (!by_count) {
-        const uint64_t w = fixed(weight(l, mx, rt));
+        const uint64_t w = weight(l, mx, rt);
         if (w) atomicAdd((unsigned long long*)&s.w[b], (unsigned long long)w);
       }
     }
@@ -137,22 +135,23 @@ __device__ Border row_border(RowLds& s, const SampleArgs& p, int t, float mx, do
         (level == 0 || (in.key >> (shift + (level == 2 ? 10 : 11))) == prefix)) {
       const int b = (in.key >> shift) & (bins - 1);
       s.n[b] += in.ties;
-      s.w[b] += in.ties * fixed(weight(key_value(in.key), mx, rt));
+      s.w[b] += in.ties * weight(key_value(in.key), mx, rt);
     }
     __syncthreads();
-    // bins from the top, two per thread; the bin in which the prefix reaches its end
-    uint64_t w[2], ws, W;
-    uint32_t n[2], ns, Nn;
-    for (int q = 0; q < 2; q++) {
-      const int b = bins - 1 - (2 * (int)threadIdx.x + q);
+    // bins from the top, some per thread; the bin in which the prefix reaches its end
+    constexpr int PER = kRowBins / kRowThreads;
+    uint64_t w[PER], ws = 0, W;
+    uint32_t n[PER], ns = 0, Nn;
+    for (int q = 0; q < PER; q++) {
+      const int b = bins - 1 - (PER * (int)threadIdx.x + q);
       w[q] = b >= 0 ? s.w[b] : 0, n[q] = b >= 0 ? s.n[b] : 0;
     }
-    ws = w[0] + w[1], ns = n[0] + n[1];
+    for (int q = 0; q < PER; q++) ws += w[q], ns += n[q];
     row_scan(s, ws, ns, W, Nn);
     if (threadIdx.x == 0) s.key = 0xffffffffu;
     __syncthreads();
-    for (int q = 0; q < 2; q++) {
-      const int b = bins - 1 - (2 * (int)threadIdx.x + q);
+    for (int q = 0; q < PER; q++) {
+      const int b = bins - 1 - (PER * (int)threadIdx.x + q);
       if (b >= 0 && n[q]) {
         const bool starts = by_count ? nabove + ns < k : (double)(wabove + ws) < want || nabove + ns == 0;
         const bool ends = by_count ? nabove + ns + n[q] >= k : (double)(wabove + ws + w[q]) >= want;
@@ -171,7 +170,7 @@ __device__ Border row_border(RowLds& s, const SampleArgs& p, int t, float mx, do
   if (by_count) {
     b.ties = k - nabove;
   } else {
-    const double w = (double)fixed(weight(key_value(prefix), mx, rt));
+    const double w = (double)weight(key_value(prefix), mx, rt);
     const double r = w > 0 ? ceil((want - (double)wabove) / w) : 1.0;
     b.ties = (uint32_t)fmin(fmax(r, 1.0), (double)have);
   }
@@ -180,7 +179,7 @@ __device__ Border row_border(RowLds& s, const SampleArgs& p, int t, float mx, do
 }
 
 template <bool BF16>
-__device__ void row_sample(RowLds& s, const SampleArgs& p, int t) {
+__device__ __attribute__((noinline)) void row_sample(RowLds& s, const SampleArgs& p, int t) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const RowPar r = row_par(p, t);
   float mx = -INFINITY;
@@ -210,7 +209,7 @@ __device__ void row_sample(RowLds& s, const SampleArgs& p, int t) {
   if (r.k < p.V) b = row_border<BF16>(s, p, t, mx, r.rt, true, (uint32_t)r.k, 0.0, Border{0, 0});
   const int parts = 64, per = (p.V + parts - 1) / parts;
   // kept weights and border ties of 64 runs of the vocabulary
-  auto sums = [&](double min_p) {
+  auto sums = [&](uint64_t min_w) {
     if (threadIdx.x < 64) s.wsum[threadIdx.x] = 0, s.nsum[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < p.V; i += kRowThreads) {
@@ -221,24 +220,22 @@ __device__ void row_sample(RowLds& s, const SampleArgs& p, int t) {
         atomicAdd(&s.nsum[i / per], 1u);
         continue;
       }
-      const double w = weight(l, mx, r.rt);
-      const uint64_t f = fixed(w);
-      if (w >= min_p && f) atomicAdd((unsigned long long*)&s.wsum[i / per], (unsigned long long)f);
+      const uint64_t f = weight(l, mx, r.rt);
+      if (f >= min_w && f) atomicAdd((unsigned long long*)&s.wsum[i / per], (unsigned long long)f);
     }
     __syncthreads();
   };
-  const uint64_t wb_all = fixed(weight(key_value(b.key), mx, r.rt));
+  const uint64_t wb_all = weight(key_value(b.key), mx, r.rt);
   if (r.top_p < 1.0) {
-    sums(0.0);
+    sums(0);
     uint64_t total = 0;
     for (int i = 0; i < parts; i++) total += s.wsum[i];
     total += b.ties * wb_all;
     __syncthreads();
     b = row_border<BF16>(s, p, t, mx, r.rt, false, 0, r.top_p * (double)total, b);
   }
-  sums(r.min_p);
-  const double wbd = weight(key_value(b.key), mx, r.rt);
-  const uint64_t wb = wbd >= r.min_p ? fixed(wbd) : 0;
+  sums(r.min_w);
+  const uint64_t wbf = weight(key_value(b.key), mx, r.rt), wb = wbf >= r.min_w ? wbf : 0;
   if (threadIdx.x == 0) {  // the run in which u times the total is passed
     uint64_t total = 0;
     uint32_t left = b.ties;
@@ -271,8 +268,8 @@ __device__ void row_sample(RowLds& s, const SampleArgs& p, int t) {
     uint32_t tie = in && key == b.key, tn = tie, N1;
     uint64_t zero = 0, W1;
     row_scan(s, zero, tn, W1, N1);  // ties before this one
-    const double wd = in ? weight(l, mx, r.rt) : 0.0;
-    uint64_t w = in && key > b.key && wd >= r.min_p ? fixed(wd) : tie && tn < left ? wb : 0, before = w, W;
+    const uint64_t f = in ? weight(l, mx, r.rt) : 0;
+    uint64_t w = in && key > b.key && f >= r.min_w ? f : tie && tn < left ? wb : 0, before = w, W;
     uint32_t dn = 0, N2;
     row_scan(s, before, dn, W, N2);
     if (w && (double)(c + before + w) > want) atomicMin(&s.at, i);
@@ -295,28 +292,28 @@ __device__ void row_sample(RowLds& s, const SampleArgs& p, int t) {
 //   k_sample_max     maxima of runs of 4, 16 or 64 logits and of tiles of 1024 (one wave each)
 //   k_sample_border  (with top-k or top-p) where the border lies, roughly. top-k: the k-th largest run maximum bounds the
 //                    k-th largest logit from below, so what lies under its bin is out. top-p: a histogram of the row over
-//                    2048 bins of (max - l) / temperature, 1/64 wide; a bin's sum is kept relative to exp at its upper
-//                    end as a whole number of 2^-12, so one 32-bit LDS addition per logit gives weights to 2^-13.
+//                    bins of (max - l) / temperature, 1/128 wide; a bin's sum is kept relative to exp at its upper end as a
+//                    whole number of 2^-12, so one 32-bit LDS addition per logit gives weights to 2^-13.
 //   k_sample_collect the tiles' sums of what is surely kept, and a list of the logits that may lie at the border
-//   k_sample_draw    one block per row sorts the list, finds the border exactly, and then the token: first its tile, from
-//                    the sums, then its place.
+//   k_sample_draw    one block per row finds the border exactly in the list, and then the token: first its tile, from the
+//                    sums, then its place.
 // The estimate only chooses what is listed: k_sample_draw checks that the exact border lies inside. Where it does not, or
-// the list is full (thousands of equal logits at the border, top_p within 4e-4 of 1 on a flat row) or top_k is past 1024,
-// it takes the one-block path above. Both give the same token.
-constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 2048, kTauBins = 1024;
-constexpr int kRowsPerLaunch = 512;
+// the list is full (thousands of equal logits at the border, top_p within 4e-4 of 1 on a flat row), top_k is past 1024 or
+// the maximum infinite, it takes the one-block path above. Both give the same token.
+constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 4096, kTauBins = 1024;
+constexpr float kBinScale = 128.f, kTauScale = 32.f;  // bins per unit of (max - l) / temperature
+constexpr int kRowsPerLaunch = 512, kSomeWaves = 8;
 
 struct RowInfo {  // what the launches of a call hand on, per row
-  uint64_t before, all;  // sums of the weights in the bins above blo, and of all
+  uint64_t before, all;  // sums of the weights in the bins above the listed ones, and of all
   uint32_t n;            // listed logits
-  int tau;               // top-k: the last bin (1/32 wide) that is listed
-  int blo, bhi;          // top-p: the bins that are listed
+  int tau;               // top-k: the last bin that is listed
 };
 struct SampleWs {
   char* base;
   size_t row;  // bytes per row: [RowInfo | list | hist | tile sums | tile maxima | run maxima]
   int tiles, runs, run;  // run: logits per run (4, 16 or 64)
-  __host__ __device__ char* at(int t) const { return base + (size_t)t * row; }
+  __device__ char* at(int t) const { return base + (size_t)t * row; }
   __device__ RowInfo* info(int t) const { return (RowInfo*)at(t); }
   __device__ uint64_t* list(int t) const { return (uint64_t*)(at(t) + 64); }
   __device__ uint32_t* hist(int t) const { return (uint32_t*)(at(t) + 64 + kList * 8); }
@@ -336,14 +333,17 @@ static SampleWs sample_ws(int V) {
 }
 
 // What a row asks for. Its filters may differ from its neighbours'.
-enum RowKind { kGreedy, kTopK, kTopP, kFull, kOneBlock };
-__device__ __forceinline__ int row_kind(const RowPar& r, int V) {
+enum RowKind { kGreedy, kTopK, kTopP, kFull, kOneBlock, kNothing };
+__device__ __forceinline__ int row_kind(const RowPar& r, int V, float mx) {
+  if (mx == -INFINITY) return kNothing;
   if (r.greedy) return kGreedy;
+  if (mx == INFINITY) return kOneBlock;
   if (r.k < V) return r.k <= kMaxK ? kTopK : kOneBlock;
   return r.top_p < 1.0 ? kTopP : kFull;
 }
 
-// The 16 logits of a lane in a tile: q's four are at 256 q + 4 lane (past V: -infinity).
+// The 16 logits of a lane in a tile: q's four are at 256 q + 4 lane (past V: -infinity). NaN stay NaN: no maximum takes them,
+// no comparison below holds for them, and their weight is 0.
 template <bool BF16>
 __device__ __forceinline__ void load_tile(const SampleArgs& p, int t, int tile, float (&l)[16]) {
   typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -356,13 +356,13 @@ __device__ __forceinline__ void load_tile(const SampleArgs& p, int t, int tile, 
 #pragma unroll
       for (int q = 0; q < 4; q++) v[q] = *(const h4*)((const uint16_t*)p.logits + row + tile * kTile + 256 * q + 4 * lane);
 #pragma unroll
-      for (int e = 0; e < 16; e++) l[e] = order_value(bf2f(v[e / 4][e % 4]));
+      for (int e = 0; e < 16; e++) l[e] = bf2f(v[e / 4][e % 4]);
     } else {
       f4 v[4];
 #pragma unroll
       for (int q = 0; q < 4; q++) v[q] = *(const f4*)((const float*)p.logits + row + tile * kTile + 256 * q + 4 * lane);
 #pragma unroll
-      for (int e = 0; e < 16; e++) l[e] = order_value(v[e / 4][e % 4]);
+      for (int e = 0; e < 16; e++) l[e] = v[e / 4][e % 4];
     }
   } else {
 #pragma unroll
@@ -386,7 +386,8 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleArgs p, SampleWs ws) {
   const int lane = threadIdx.x & 63, t = blockIdx.y, tile = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (blockIdx.x == 0) {
     uint32_t* const h = ws.hist(t);
-    for (int i = threadIdx.x; i < kBins; i += 256) h[i] = 0;
+    if (p.top_p)
+      for (int i = threadIdx.x; i < kBins; i += 256) h[i] = 0;
     if (threadIdx.x == 0) *ws.info(t) = RowInfo{};
   }
   if (tile >= ws.tiles) return;
@@ -429,28 +430,29 @@ __device__ __forceinline__ float row_max(const SampleWs& ws, int t, float* s) {
   for (int i = 1; i < W; i++) m = fmaxf(m, s[i]);
   return m;
 }
-// (max - l) / temperature in bins of 1 / scale, the last of which holds all that is left; monotone in l
-__device__ __forceinline__ float bin_of(float l, float mx, float rt_scale, int bins) {
-  return l == mx ? 0.f : fminf((mx - l) * rt_scale, (float)(bins - 1));
+// Bins per unit of the logits (finite, so that the maximum itself is in bin 0; log2(e) is taken out of rt again).
+__device__ __forceinline__ float bin_scale(const RowPar& r, float scale) {
+  return (float)fmin(r.rt * 0.69314718055994531 * scale, 3e38);
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(256) void k_sample_border(SampleArgs p, SampleWs ws) {
+__global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p, SampleWs ws) {
   __shared__ uint32_t h[kBins];
-  __shared__ float s[4];
+  __shared__ float s[kSomeWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
   const RowPar r = row_par(p, t);
-  const int kind = row_kind(r, p.V);
+  // (a maximum above -infinity and below infinity: whether it is that comes after the rows that have no work here)
+  int kind = row_kind(r, p.V, 0.f);
   if (kind != kTopP && !(kind == kTopK && blockIdx.x == 0)) return;
-  for (int i = threadIdx.x; i < kBins; i += 256) h[i] = 0;
-  const float mx = row_max<4>(ws, t, s);  // with a barrier
-  if (mx == -INFINITY) return;
+  for (int i = threadIdx.x; i < (kind == kTopK ? kTauBins : kBins); i += 64 * kSomeWaves) h[i] = 0;
+  const float mx = row_max<kSomeWaves>(ws, t, s);  // with a barrier
+  if (row_kind(r, p.V, mx) != kind) return;
   if (kind == kTopK) {
-    const float sc = (float)(r.rt * 32.0);
+    const float sc = bin_scale(r, kTauScale);
     const float* const rm = ws.rmax(t);
-    for (int i = threadIdx.x; i < ws.runs; i += 256) {
-      const int b = (int)bin_of(rm[i], mx, sc, kTauBins);
-      if (b < kTauBins - 1) atomicAdd(&h[b], 1u);
+    for (int i = threadIdx.x; i < ws.runs; i += 64 * kSomeWaves) {
+      const float y = (mx - rm[i]) * sc;
+      if (y < (float)(kTauBins - 1)) atomicAdd(&h[(int)y], 1u);
     }
     __syncthreads();
     if (wave == 0) {  // the first bin at which k runs have been seen; without one, all that has a weight
@@ -475,33 +477,37 @@ __global__ __launch_bounds__(256) void k_sample_border(SampleArgs p, SampleWs ws
     }
     return;
   }
-  const float sc = (float)(r.rt * 64.0);
-  for (int tile = blockIdx.x * 4 + wave; tile < ws.tiles; tile += 4 * gridDim.x) {
+  const float sc = bin_scale(r, kBinScale);
+  for (int tile = blockIdx.x * kSomeWaves + wave; tile < ws.tiles; tile += kSomeWaves * gridDim.x) {
     float l[16];
     load_tile<BF16>(p, t, tile, l);
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-      const float y = bin_of(l[e], mx, sc, kBins);
-      const int b = (int)y;
-      const float f = y - (float)b;
-      // exp(-f / 64) to 1e-6
-      if (b < kBins - 1) atomicAdd(&h[b], (uint32_t)(4096.5f + f * (-64.f + 0.5f * f)));
+      const float y = (mx - l[e]) * sc;
+      if (y < (float)(kBins - 1)) {  // beyond: no weight
+        const int b = (int)y;
+        const float f = y - (float)b;
+        // 4096 exp(-f / 128), to 1e-7
+        atomicAdd(&h[b], (uint32_t)__builtin_fmaf(f, __builtin_fmaf(f, 0.125f, -32.f), 4096.5f));
+      }
     }
   }
   __syncthreads();
   uint32_t* const g = ws.hist(t);
-  for (int i = threadIdx.x; i < kBins; i += 256)
+  for (int i = threadIdx.x; i < kBins; i += 64 * kSomeWaves)
     if (h[i]) atomicAdd(&g[i], h[i]);
 }
 
-// The bins in which the border of top-p may lie: the histogram's sums are within 1.4e-4, and lo and hi 4e-4 off.
+// The first and last bin in which the border of top-p may lie: the histogram's sums are within 1.4e-4 of the weights', and
+// the sought ones 4e-4 off to either side.
 __device__ __forceinline__ void top_p_bins(const uint32_t* g, double top_p, double* part, int* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double w[8], own = 0;
+  constexpr int PER = kBins / (64 * kSomeWaves);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = PER * (int)threadIdx.x;
+  float w[PER];
+  double own = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int b = 8 * (int)threadIdx.x + i;
-    w[i] = (double)g[b] * (double)expf((float)b * -0.015625f);
+  for (int i = 0; i < PER; i++) {
+    w[i] = (float)g[b0 + i] * __builtin_amdgcn_exp2f((float)(b0 + i) * (-1.44269504f / kBinScale));
     own += w[i];
   }
   double c = own;
@@ -515,89 +521,99 @@ __device__ __forceinline__ void top_p_bins(const uint32_t* g, double top_p, doub
   __syncthreads();
   double all = 0, base = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < kSomeWaves; i++) {
     if (i == wave) base = all;
     all += part[i];
   }
-  double x = base + c - own;
+  const double x = base + c - own;
 #pragma unroll
   for (int k = 0; k < 2; k++) {
     const double want = top_p * all * (k ? 1 + 4e-4 : 1 - 4e-4);
-    double y = x;
-    int at;
-#pragma unroll
-    for (int i = 7; i >= 0; i--) y += w[i];  // (this thread's end)
-    if (y >= want) {
-      y = x, at = 8 * (int)threadIdx.x + 7;
-      for (int i = 0; i < 7; i++) {
+    if (x + own >= want && (x < want || threadIdx.x == 0)) {
+      double y = x;
+      int i = 0;
+      for (; i < PER - 1; i++) {
         y += w[i];
-        if (y >= want) {
-          at = 8 * (int)threadIdx.x + i;
-          break;
-        }
+        if (y >= want) break;
       }
-      atomicMin(&out[k], at);
+      atomicMin(&out[k], b0 + i);
     }
   }
   __syncthreads();
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(256) void k_sample_collect(SampleArgs p, SampleWs ws) {
-  __shared__ float s[4];
-  __shared__ double part[4];
+__global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p, SampleWs ws) {
+  __shared__ float s[kSomeWaves];
+  __shared__ double part[kSomeWaves];
   __shared__ int bins[2];
+  __shared__ uint64_t found[kList];  // this block's part of the list (a global atomic per entry costs its latency)
+  __shared__ uint32_t nfound, at0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
   const RowPar r = row_par(p, t);
-  const int kind = row_kind(r, p.V);
-  if (kind == kGreedy || kind == kOneBlock) return;
-  const float mx = row_max<4>(ws, t, s);
-  if (mx == -INFINITY) return;
+  if (r.greedy) return;
+  const float mx = row_max<kSomeWaves>(ws, t, s);
+  const int kind = row_kind(r, p.V, mx);
+  if (kind != kTopK && kind != kTopP && kind != kFull) return;
   RowInfo* const info = ws.info(t);
-  uint64_t* const list = ws.list(t);
-  // bins (of 1 / 32 for top-k) up to `sure` are kept whole, and those up to `last` listed
-  int sure = kBins, last = -1;
-  float sc = (float)(r.rt * 64.0);
+  if (threadIdx.x == 0) nfound = 0;
+  __syncthreads();
+  // y = (max - l) scale: below `sure` kept whole, from there to below `last` listed
+  float sure = INFINITY, last = INFINITY, sc = 0.f;
   if (kind == kTopK) {
-    sure = -1, last = info->tau, sc = (float)(r.rt * 32.0);
+    sure = 0.f, last = (float)(info->tau + 1), sc = bin_scale(r, kTauScale);
   } else if (kind == kTopP) {
     top_p_bins(ws.hist(t), r.top_p, part, bins);
-    sure = bins[0] - 1, last = bins[1];
-    if (blockIdx.x == 0 && threadIdx.x == 0) info->blo = bins[0], info->bhi = bins[1];
+    sure = (float)bins[0], last = (float)(bins[1] + 1), sc = bin_scale(r, kBinScale);
   }
-  const int nbins = kind == kTopK ? kTauBins : kBins;
-  uint64_t before = 0, all = 0;
-  for (int tile = blockIdx.x * 4 + wave; tile < ws.tiles; tile += 4 * gridDim.x) {
-    float l[16];
-    load_tile<BF16>(p, t, tile, l);
-    uint64_t keep = 0;
+  auto add_to_list = [&](int tile, const float (&l)[16], const float (&y)[16]) {
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-      const int b = (int)bin_of(l[e], mx, sc, nbins);
-      if (kind != kTopK) {
-        const double w = weight(l[e], mx, r.rt);
-        const uint64_t f = fixed(w);
-        all += f;
-        if (b <= sure) {
-          before += f;
-          keep += w >= r.min_p ? f : 0;
-        }
-      }
-      const bool add = b > sure && b <= last && l[e] != -INFINITY;
+      const bool add = y[e] >= sure && y[e] < last;
       const uint64_t who = __ballot(add);
       if (who) {
         uint32_t at = 0;
-        if (lane == __ffsll((long long)who) - 1) at = atomicAdd(&info->n, (uint32_t)__popcll(who));
+        if (lane == __ffsll((long long)who) - 1) at = atomicAdd(&nfound, (uint32_t)__popcll(who));
         at = (uint32_t)__builtin_amdgcn_readlane((int)at, __ffsll((long long)who) - 1);
         at += (uint32_t)__popcll(who & ((1ull << lane) - 1));
         if (add && at < kList)
-          list[at] = (uint64_t)~order_key(l[e]) << 32 | (uint32_t)(tile * kTile + tile_at(e));
+          found[at] = (uint64_t)~order_key(l[e]) << 32 | (uint32_t)(tile * kTile + tile_at(e));
       }
     }
-    if (kind != kTopK) {
-      keep = wave_sum_u64(keep);
-      if (lane == 0) ws.tsum(t)[tile] = keep;
+  };
+  uint64_t before = 0, all = 0;
+  for (int tile = blockIdx.x * kSomeWaves + wave; tile < ws.tiles; tile += kSomeWaves * gridDim.x) {
+    float l[16], y[16];
+    if (kind == kTopK && (mx - ws.tmax(t)[tile]) * sc >= last) continue;
+    load_tile<BF16>(p, t, tile, l);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      y[e] = kind == kFull ? 0.f : (mx - l[e]) * sc;
+      any |= y[e] >= sure && y[e] < last;
     }
+    if (__ballot(any)) add_to_list(tile, l, y);
+    if (kind == kTopK) continue;
+    // sums of what is above the listed bins, and of that with min_p; of all
+    uint64_t in = 0, keep = 0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const uint64_t f = exp2_fixed44(((double)l[e] - (double)mx) * r.rt), g = y[e] < sure ? f : 0;
+      all += f;
+      in += g;
+      if (r.min_w) keep += g >= r.min_w ? g : 0;
+    }
+    before += in;
+    keep = wave_sum_u64(r.min_w ? keep : in);
+    if (lane == 0) ws.tsum(t)[tile] = keep;
+  }
+  __syncthreads();
+  const uint32_t n = nfound;
+  if (n) {
+    if (threadIdx.x == 0) at0 = atomicAdd(&info->n, n);
+    __syncthreads();
+    uint64_t* const list = ws.list(t);
+    for (uint32_t i = threadIdx.x; i < n && at0 + i < kList; i += 64 * kSomeWaves) list[at0 + i] = found[i];
   }
   if (kind == kTopP) {
     before = wave_sum_u64(before), all = wave_sum_u64(all);
@@ -625,175 +641,267 @@ __device__ __forceinline__ void sort_lds(uint64_t* a, int n) {
     }
 }
 
+constexpr int kSub = kRowThreads;  // sub-bins of the list's range, one per thread
 struct DrawLds {
   union {
     RowLds row;
     struct {
-      uint64_t a[kList];
-      uint64_t w[kMaxK];
+      uint64_t few[kList];  // the entries of the border's sub-bin
+      uint64_t w[kSub];
       uint64_t tile[kSampleMaxV / kTile];
+      uint32_t n[kSub];
     } f;
   };
-  uint64_t wpart[16];
-  uint32_t npart[16];
-  float s[16];
-  uint64_t border;
-  int at, ok;
+  uint64_t wpart[kRowThreads / 64];
+  uint32_t npart[kRowThreads / 64];
+  float s[kRowThreads / 64];
+  uint64_t border, base;
+  float range[2];
+  int at, ok, bin, nfew;
 };
 
-// Exclusive block-wide prefix of w by thread; the total in W.
-__device__ __forceinline__ uint64_t draw_scan(DrawLds& s, uint64_t w, uint64_t& W) {
+// Exclusive block-wide prefix of (w, n) by thread; the totals in W and Nn.
+__device__ __forceinline__ void draw_scan(DrawLds& s, uint64_t& w, uint32_t& n, uint64_t& W, uint32_t& Nn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint64_t c = w;
+  uint32_t d = n;
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
     const uint64_t a = __shfl_up(c, o, 64);
-    if (lane >= o) c += a;
+    const uint32_t b = __shfl_up(d, o, 64);
+    if (lane >= o) c += a, d += b;
   }
   __syncthreads();
-  if (lane == 63) s.wpart[wave] = c;
+  if (lane == 63) s.wpart[wave] = c, s.npart[wave] = d;
   __syncthreads();
   uint64_t base = 0;
-  W = 0;
+  uint32_t bn = 0;
+  W = 0, Nn = 0;
   for (int i = 0; i < kRowThreads / 64; i++) {
-    if (i == wave) base = W;
-    W += s.wpart[i];
+    if (i == wave) base = W, bn = Nn;
+    W += s.wpart[i], Nn += s.npart[i];
   }
-  return base + c - w;
+  w = base + c - w, n = bn + d - n;
 }
+
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+// A list entry: ~key in the upper half, its place in the vocabulary in the lower, so that rising entries are the order.
+__device__ __forceinline__ float entry_logit(uint64_t a) { return key_value(~(uint32_t)(a >> 32)); }
 
 template <bool BF16>
 __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, SampleWs ws) {
   __shared__ DrawLds s;
-  const int t = blockIdx.x, tid = threadIdx.x;
+  constexpr int PER = kList / kRowThreads;
+  static_assert(kSampleMaxV / kTile <= kRowThreads, "a tile per thread");
+  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  // loads that depend on nothing, together (a row's draw is a chain of memory latencies)
   const RowPar r = row_par(p, t);
-  const int kind = row_kind(r, p.V);
-  const float mx = row_max<16>(ws, t, s.s);
+  const RowInfo in = *ws.info(t);
+  const float tile_max = tid < ws.tiles ? ws.tmax(t)[tid] : -INFINITY;
+  const uint64_t tile_sum = tid < ws.tiles ? ws.tsum(t)[tid] : 0;
+  uint64_t a[PER], f[PER];
+  a[0] = ws.list(t)[tid];
   const double u = row_u(p, t);
-  if (tid == 0) s.at = 0x7fffffff, s.ok = 1;
+  float mx = dpp_max_f(tile_max);
+  if (lane == 0) s.s[tid >> 6] = mx;
+  if (tid == 0) s.at = 0x7fffffff;
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRowThreads / 64; i++) mx = fmaxf(mx, s.s[i]);
+  const int kind = row_kind(r, p.V, mx);
   auto done = [&](int token, float prob) {
     p.token[t] = token;
     if (p.prob) p.prob[t] = prob;
   };
-  if (mx == -INFINITY) {
+  if (kind == kNothing) {
     if (tid == 0) done(-1, 0.f);
     return;
   }
   if (kind == kGreedy) {  // the first tile with the maximum, and its place there
-    for (int i = tid; i < ws.tiles; i += kRowThreads)
-      if (ws.tmax(t)[i] == mx) atomicMin(&s.at, i);
+    if (tile_max == mx) atomicMin(&s.at, tid);
     __syncthreads();
-    const int i = s.at * kTile + tid;
+    const int first = s.at * kTile;
     __syncthreads();
     if (tid == 0) s.at = 0x7fffffff;
     __syncthreads();
-    if (i < p.V && load_logit<BF16>(p, t, i) == mx) atomicMin(&s.at, i);
+    for (int i = first + tid; i < min(first + kTile, p.V); i += kRowThreads)
+      if (load_logit<BF16>(p, t, i) == mx) atomicMin(&s.at, i);
     __syncthreads();
     if (tid == 0) done(s.at, 1.f);
     return;
   }
-  RowInfo in = *ws.info(t);
   const int n = (int)min(in.n, (uint32_t)kList + 1);
-  if (kind == kOneBlock || n > kList) {
+  bool listed = kind != kOneBlock && n <= kList;
+  // what is kept: the prefix of the order up to the entry `border`, as far as it has min_p
+  uint64_t border = ~0ull;
+  int sub[PER];
+  if (listed && kind != kFull) {
+    // the list in registers, over 512 sub-bins of its range of logits
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < PER; q++) {
+      const int i = kRowThreads * q + tid;
+      if (q > 0 && kRowThreads * q < n) a[q] = ws.list(t)[min(i, n - 1)];
+      if (i >= n) a[q] = 0;
+      const float l = entry_logit(a[q]);
+      f[q] = i < n ? weight(l, mx, r.rt) : 0;
+      if (i < n) lo = fminf(lo, l), hi = fmaxf(hi, l);
+    }
+    lo = -dpp_max_f(-lo), hi = dpp_max_f(hi);
+    if (lane == 0) s.npart[tid >> 6] = __float_as_uint(lo), s.s[tid >> 6] = hi;
+    s.f.w[tid] = 0, s.f.n[tid] = 0;
     __syncthreads();
+    lo = INFINITY, hi = -INFINITY;
+    for (int i = 0; i < kRowThreads / 64; i++) lo = fminf(lo, __uint_as_float(s.npart[i])), hi = fmaxf(hi, s.s[i]);
+    const float sc = hi > lo ? fminf((float)(kSub - 1) / (hi - lo), 3e38f) : 0.f;
+#pragma unroll
+    for (int q = 0; q < PER; q++) {
+      sub[q] = -1;
+      if (kRowThreads * q + tid < n) {
+        sub[q] = min((int)((hi - entry_logit(a[q])) * sc), kSub - 1);
+        atomicAdd(&s.f.n[sub[q]], 1u);
+        if (f[q]) atomicAdd((unsigned long long*)&s.f.w[sub[q]], (unsigned long long)f[q]);
+      }
+    }
+    __syncthreads();
+    const uint64_t own_w = s.f.w[tid];
+    const uint32_t own_n = s.f.n[tid];
+    const uint32_t k = (uint32_t)min(r.k, n);
+    uint64_t bw = own_w, W;
+    uint32_t bn = own_n, Nn;
+    draw_scan(s, bw, bn, W, Nn);  // this thread's sub-bin: what comes before it
+    if (tid < ws.tiles) s.f.tile[tid] = kind == kTopP ? tile_sum : 0;
+    // The border by count (top-k: the k-th entry, or the last), then by weight (the first entry at which the sum reaches want, `base`
+    // before the list): its sub-bin, and there, among few, the entry.
+#pragma clang loop unroll(disable)
+    for (int step = 0; step < 2; step++) {
+      const bool by_count = step == 0;
+      if (by_count ? kind != kTopK : r.top_p >= 1.0) continue;
+      const uint64_t base = kind == kTopP ? in.before : 0;
+      double want = 0;
+      if (!by_count) {
+        uint64_t all = in.all;
+        if (kind == kTopK) {
+          uint64_t mine = 0;
+          uint32_t z = 0, zz;
+#pragma unroll
+          for (int q = 0; q < PER; q++) mine += sub[q] >= 0 && a[q] <= border ? f[q] : 0;
+          draw_scan(s, mine, z, all, zz);
+        }
+        want = r.top_p * (double)all;
+        // the border lies above what is listed, or below
+        listed = (base == 0 || (double)base < want) && (double)(base + W) >= want;
+        if (!listed) break;
+      }
+      if (tid == 0) s.bin = kSub - 1, s.nfew = 0;
+      __syncthreads();
+      if (own_n) {
+        const bool here = by_count ? bn < k && bn + own_n >= k
+                                   : ((double)(base + bw) < want || base + bw == 0) && (double)(base + bw + own_w) >= want;
+        if (here) s.bin = tid;
+      }
+      __syncthreads();
+      const int bin = s.bin;
+      if (tid == bin) s.base = base + bw, s.npart[0] = bn;
+#pragma unroll
+      for (int q = 0; q < PER; q++)
+        if (sub[q] == bin) s.f.few[atomicAdd(&s.nfew, 1)] = a[q];
+      __syncthreads();
+      const int m = s.nfew;
+      if (m > 64) sort_lds(s.f.few, m);
+      if (tid < 64) {
+        uint64_t c = s.base;
+        uint32_t d = s.npart[0];
+        uint64_t at = ~0ull;
+        for (int i0 = 0; i0 < m && at == ~0ull; i0 += 64) {  // 64 entries at a time: unsorted if there are no more
+          const bool live = i0 + lane < m;
+          const uint64_t x = live ? s.f.few[i0 + lane] : ~0ull;
+          const uint64_t w = live ? weight(entry_logit(x), mx, r.rt) : 0;
+          uint64_t before = c;
+          uint32_t rank = d;
+          for (int j = 0; j < min(m - i0, 64); j++) {
+            const uint64_t y = readlane_u64(x, j), v = readlane_u64(w, j);
+            if (y < x) before += v, rank++;
+            c += v;
+          }
+          d += min(m - i0, 64);
+          const bool hit = live && (by_count ? rank == k - 1
+                                             : ((double)before < want || before == 0) && (double)(before + w) >= want);
+          const uint64_t who = __ballot(hit);
+          if (who) at = readlane_u64(x, __ffsll((long long)who) - 1);
+        }
+        if (lane == 0) s.border = at;
+      }
+      __syncthreads();
+      border = s.border < border ? s.border : border;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; q++)
+      if (sub[q] >= 0 && a[q] <= border && f[q] && f[q] >= r.min_w)
+        atomicAdd((unsigned long long*)&s.f.tile[(uint32_t)a[q] / kTile], (unsigned long long)f[q]);
+  } else if (listed) {
+    if (tid < ws.tiles) s.f.tile[tid] = tile_sum;
+  }
+  __syncthreads();
+  if (!listed) {
     row_sample<BF16>(s.row, p, t);
     return;
   }
-  auto entry_key = [](uint64_t a) { return ~(uint32_t)(a >> 32); };
-  if (kind == kTopK) {
-    for (int i = tid; i < n; i += kRowThreads) s.f.a[i] = ws.list(t)[i];
-    sort_lds(s.f.a, n);
-    // thread i: the i-th largest of the first k <= 1024
-    const bool in_k = tid < min(n, r.k);
-    const uint64_t a = s.f.a[in_k ? tid : 0];
-    const double wd = in_k ? weight(key_value(entry_key(a)), mx, r.rt) : 0.0;
-    const uint64_t w = in_k ? fixed(wd) : 0;
-    uint64_t all, total, before = draw_scan(s, w, all);
-    const bool in_p = r.top_p >= 1.0 || tid == 0 || (double)before < r.top_p * (double)all;
-    const uint64_t f = in_k && in_p && wd >= r.min_p ? w : 0;
-    draw_scan(s, f, total);
-    // in the order of the vocabulary
-    const int m = min(n, r.k);
-    s.f.w[tid] = f;
-    __syncthreads();
-    if (tid < m) s.f.a[tid] = (a & 0xffffffffu) << 32 | (uint32_t)tid;
-    __syncthreads();
-    sort_lds(s.f.a, m);
-    const uint64_t b = s.f.a[tid < m ? tid : 0];
-    const uint64_t fw = tid < m ? s.f.w[(uint32_t)b] : 0;
-    uint64_t W;
-    before = draw_scan(s, fw, W);
-    if (fw && (double)(before + fw) > u * (double)total) atomicMin(&s.at, tid);
-    __syncthreads();
-    if (tid == s.at) done((int)(b >> 32), (float)((double)fw / (double)total));
-    return;
-  }
-  // kept: what comes before or at the border entry in the order, and has min_p
-  uint64_t border = ~0ull;
-  for (int i = tid; i < ws.tiles; i += kRowThreads) s.f.tile[i] = ws.tsum(t)[i];
-  if (kind == kTopP) {
-    for (int i = tid; i < n; i += kRowThreads) s.f.a[i] = ws.list(t)[i];
-    sort_lds(s.f.a, n);
-    const double want = r.top_p * (double)in.all;
-    if (in.before != 0 && !((double)in.before < want)) s.ok = 0;  // the border lies above what is listed
-    if (tid == 0) s.border = 0;
-    uint64_t c = in.before;
-    for (int i0 = 0; i0 < n; i0 += kRowThreads) {
-      const int i = i0 + tid;
-      const uint64_t a = s.f.a[min(i, n - 1)];
-      const double wd = i < n ? weight(key_value(entry_key(a)), mx, r.rt) : 0.0;
-      const uint64_t w = fixed(wd);
-      uint64_t W;
-      const uint64_t before = c + draw_scan(s, w, W);
-      if (i < n && ((double)before < want || before == 0)) {
-        if (i == 0 || before != 0) atomicMax((unsigned long long*)&s.border, (unsigned long long)a);
-        if (wd >= r.min_p && (i == 0 || before != 0))
-          atomicAdd((unsigned long long*)&s.f.tile[(uint32_t)a / kTile], (unsigned long long)w);
-      }
-      c += W;
-    }
-    if ((double)c < want) s.ok = 0;  // or below
-    __syncthreads();
-    border = s.border;
-    if (!s.ok) {
-      __syncthreads();
-      row_sample<BF16>(s.row, p, t);
-      return;
-    }
-  }
-  __syncthreads();
   uint64_t total, W;
+  uint32_t z = 0, zz;
   const uint64_t mine = tid < ws.tiles ? s.f.tile[tid] : 0;
-  uint64_t before = draw_scan(s, mine, total);
+  uint64_t before = mine;
+  draw_scan(s, before, z, total, zz);
   const double want = u * (double)total;
   if (mine && (double)(before + mine) > want) atomicMin(&s.at, tid);
   __syncthreads();
   const int tile = min(s.at, ws.tiles - 1);
-  if (tid == tile) s.border = before;
+  if (tid == tile) s.base = before;
   __syncthreads();
-  const uint64_t base = s.border;
+  const uint64_t base = s.base;
   if (tid == 0) s.at = 0x7fffffff;
-  const int i = tile * kTile + tid;
-  const float l = i < p.V ? load_logit<BF16>(p, t, i) : -INFINITY;
-  const double wd = i < p.V ? weight(l, mx, r.rt) : 0.0;
-  const uint64_t a = (uint64_t)~order_key(l) << 32 | (uint32_t)i;
-  const uint64_t f = a <= border && wd >= r.min_p ? fixed(wd) : 0;
-  before = base + draw_scan(s, f, W);
-  if (f && (double)(before + f) > want) atomicMin(&s.at, i);
+  constexpr int RUN = kTile / kRowThreads;  // neighbouring logits per thread
+  const int i0 = tile * kTile + RUN * tid;
+  uint64_t fx[RUN];
+  before = 0;
+#pragma unroll
+  for (int q = 0; q < RUN; q++) {
+    const int i = i0 + q;
+    const float l = load_logit<BF16>(p, t, min(i, p.V - 1));
+    const uint64_t e = (uint64_t)~order_key(l) << 32 | (uint32_t)i;
+    const uint64_t w = weight(l, mx, r.rt);
+    fx[q] = i < p.V && e <= border && w >= r.min_w ? w : 0;
+    before += fx[q];
+  }
+  z = 0;
+  draw_scan(s, before, z, W, zz);
+  before += base;
+  int at = 0x7fffffff;
+  uint64_t fat = 0;
+#pragma unroll
+  for (int q = 0; q < RUN; q++) {
+    before += fx[q];
+    if (fx[q] && (double)before > want && at == 0x7fffffff) at = i0 + q, fat = fx[q];
+  }
+  if (fat) atomicMin(&s.at, at);
   __syncthreads();
-  if (i == s.at) done(i, (float)((double)f / (double)total));
+  if (fat && at == s.at) done(at, (float)((double)fat / (double)total));
 }
 
 size_t sample_workspace(int T, int V) { return (size_t)std::min(T, kRowsPerLaunch) * sample_ws(V).row; }
 
 template <bool BF16>
 static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream_t st) {
-  const int quads = (ws.tiles + 3) / 4;
-  const dim3 block(256), grid(quads, a.T), some(std::min(quads, std::max(1, 1024 / a.T)), a.T);
-  hipLaunchKernelGGL(k_sample_max<BF16>, grid, block, 0, st, a, ws);
-  if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some, block, 0, st, a, ws);
-  hipLaunchKernelGGL(k_sample_collect<BF16>, some, block, 0, st, a, ws);
+  const auto blocks = [&](int waves) { return (ws.tiles + waves - 1) / waves; };
+  // a wave per tile where that does not fill the device; past it fewer blocks, which set up or join a histogram each
+  const dim3 some(std::min(blocks(kSomeWaves), std::max(1, 512 / a.T)), a.T), some_threads(64 * kSomeWaves);
+  hipLaunchKernelGGL(k_sample_max<BF16>, dim3(blocks(4), a.T), dim3(256), 0, st, a, ws);
+  if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some, some_threads, 0, st, a, ws);
+  hipLaunchKernelGGL(k_sample_collect<BF16>, some, some_threads, 0, st, a, ws);
   hipLaunchKernelGGL(k_sample_draw<BF16>, dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
   return check_launch("sample");
 }
