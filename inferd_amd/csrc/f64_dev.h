@@ -58,30 +58,56 @@ __device__ __forceinline__ double rcp64(double d) {
   return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
-// A DPP move of both halves (lanes without a source keep `id`).
+// 64-bit values across lanes. A DPP move of both halves (lanes without a source get `id`):
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_u64(uint64_t id, uint64_t v) {
+  const u32x2 i = __builtin_bit_cast(u32x2, id), u = __builtin_bit_cast(u32x2, v);
+  u32x2 r;
+  r[0] = (uint32_t)__builtin_amdgcn_update_dpp((int)i[0], (int)u[0], CTRL, ROWS, 0xf, false);
+  r[1] = (uint32_t)__builtin_amdgcn_update_dpp((int)i[1], (int)u[1], CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(uint64_t, r);
+}
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dpp_f64(double id, double v) {
-  const uint64_t i = __builtin_bit_cast(uint64_t, id), u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)i, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(i >> 32), (int)(u >> 32), CTRL, ROWS, 0xf, false);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  return __builtin_bit_cast(double, dpp_u64<CTRL, ROWS>(__builtin_bit_cast(uint64_t, id), __builtin_bit_cast(uint64_t, v)));
+}
+__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int lane) {
+  const u32x2 u = __builtin_bit_cast(u32x2, v);
+  u32x2 r;
+  r[0] = (uint32_t)__builtin_amdgcn_readlane((int)u[0], lane);
+  r[1] = (uint32_t)__builtin_amdgcn_readlane((int)u[1], lane);
+  return __builtin_bit_cast(uint64_t, r);
 }
 __device__ __forceinline__ double readlane_f64(double v, int lane) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  return __builtin_bit_cast(double, readlane_u64(__builtin_bit_cast(uint64_t, v), lane));
 }
-// Wave-wide sum, the same order in every call (see dpp_reduce_i).
-__device__ __forceinline__ double dpp_sum_f64(double v) {
+// Inclusive prefix sums over a wave (the steps of dpp_reduce_i, which leave each lane the sum up to it).
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
+  v += dpp_u64<0x111, 0xf>(0, v);
+  v += dpp_u64<0x112, 0xf>(0, v);
+  v += dpp_u64<0x114, 0xf>(0, v);
+  v += dpp_u64<0x118, 0xf>(0, v);
+  v += dpp_u64<0x142, 0xa>(0, v);
+  return v + dpp_u64<0x143, 0xc>(0, v);
+}
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
   v += dpp_f64<0x111, 0xf>(0.0, v);
   v += dpp_f64<0x112, 0xf>(0.0, v);
   v += dpp_f64<0x114, 0xf>(0.0, v);
   v += dpp_f64<0x118, 0xf>(0.0, v);
   v += dpp_f64<0x142, 0xa>(0.0, v);
-  v += dpp_f64<0x143, 0xc>(0.0, v);
-  return readlane_f64(v, 63);
+  return v + dpp_f64<0x143, 0xc>(0.0, v);
 }
+__device__ __forceinline__ double dpp_sum_f64(double v) { return readlane_f64(wave_scan_f64(v), 63); }
+__device__ __forceinline__ uint64_t dpp_sum_u64(uint64_t v) { return readlane_u64(wave_scan_u64(v), 63); }
 
 // Unsigned keys in the order of the values; -0 as +0, NaN as -infinity.
 __device__ __forceinline__ float order_value(float v) { return v != v ? -INFINITY : v + 0.f; }

@@ -80,14 +80,8 @@ struct RowLds {
 // Block-wide exclusive prefix of (w, n) by thread; the totals in W, Nn.
 __device__ __forceinline__ void row_scan(RowLds& s, uint64_t& w, uint32_t& n, uint64_t& W, uint32_t& Nn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t iw = w;
-  uint32_t in = n;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const uint64_t a = __shfl_up(iw, o, 64);
-    const uint32_t b = __shfl_up(in, o, 64);
-    if (lane >= o) iw += a, in += b;
-  }
+  const uint64_t iw = wave_scan_u64(w);
+  const uint32_t in = wave_scan_u32(n);
   __syncthreads();
   if (lane == 63) s.wpart[wave] = iw, s.npart[wave] = in;
   __syncthreads();
@@ -302,7 +296,7 @@ __device__ __attribute__((noinline)) void row_sample(RowLds& s, const SampleArgs
 // the maximum infinite, it takes the one-block path above. Both give the same token.
 constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 4096, kTauBins = 1024;
 constexpr float kBinScale = 128.f, kTauScale = 32.f;  // bins per unit of (max - l) / temperature
-constexpr int kRowsPerLaunch = 512, kSomeWaves = 8;
+constexpr int kRowsPerLaunch = 512, kSomeWaves = 8, kCollect = 768;
 
 struct RowInfo {  // what the launches of a call hand on, per row
   uint64_t before, all;  // sums of the weights in the bins above the listed ones, and of all
@@ -374,12 +368,6 @@ __device__ __forceinline__ void load_tile(const SampleArgs& p, int t, int tile, 
   }
 }
 __device__ __forceinline__ int tile_at(int e) { return 256 * (e / 4) + 4 * (int)(threadIdx.x & 63) + e % 4; }
-
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) v += __shfl_xor(v, o, 64);
-  return v;
-}
 
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_sample_max(SampleArgs p, SampleWs ws) {
@@ -459,12 +447,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p,
       uint32_t n[16], own = 0;
 #pragma unroll
       for (int i = 0; i < 16; i++) own += n[i] = h[16 * lane + i];
-      uint32_t c = own;
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) {
-        const uint32_t a = __shfl_up(c, o, 64);
-        if (lane >= o) c += a;
-      }
+      const uint32_t c = wave_scan_u32(own);
       const uint64_t hit = __ballot(c >= (uint32_t)r.k);
       if (hit == 0) {
         if (lane == 0) ws.info(t)->tau = kTauBins - 2;
@@ -510,12 +493,7 @@ __device__ __forceinline__ void top_p_bins(const uint32_t* g, double top_p, doub
     w[i] = (float)g[b0 + i] * __builtin_amdgcn_exp2f((float)(b0 + i) * (-1.44269504f / kBinScale));
     own += w[i];
   }
-  double c = own;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const double a = __shfl_up(c, o, 64);
-    if (lane >= o) c += a;
-  }
+  const double c = wave_scan_f64(own);
   if (lane == 63) part[wave] = c;
   if (threadIdx.x == 0) out[0] = out[1] = kBins - 2;  // (nothing in the last bin has a weight)
   __syncthreads();
@@ -604,7 +582,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p
       if (r.min_w) keep += g >= r.min_w ? g : 0;
     }
     before += in;
-    keep = wave_sum_u64(r.min_w ? keep : in);
+    keep = dpp_sum_u64(r.min_w ? keep : in);
     if (lane == 0) ws.tsum(t)[tile] = keep;
   }
   __syncthreads();
@@ -616,7 +594,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p
     for (uint32_t i = threadIdx.x; i < n && at0 + i < kList; i += 64 * kSomeWaves) list[at0 + i] = found[i];
   }
   if (kind == kTopP) {
-    before = wave_sum_u64(before), all = wave_sum_u64(all);
+    before = dpp_sum_u64(before), all = dpp_sum_u64(all);
     if (lane == 0) {
       if (before) atomicAdd((unsigned long long*)&info->before, (unsigned long long)before);
       if (all) atomicAdd((unsigned long long*)&info->all, (unsigned long long)all);
@@ -655,22 +633,15 @@ struct DrawLds {
   uint64_t wpart[kRowThreads / 64];
   uint32_t npart[kRowThreads / 64];
   float s[kRowThreads / 64];
-  uint64_t border, base;
-  float range[2];
-  int at, ok, bin, nfew;
+  uint64_t border, base, upto;  // upto: the sum of the weights up to the border entry
+  int at, bin, nfew;
 };
 
 // Exclusive block-wide prefix of (w, n) by thread; the totals in W and Nn.
 __device__ __forceinline__ void draw_scan(DrawLds& s, uint64_t& w, uint32_t& n, uint64_t& W, uint32_t& Nn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t c = w;
-  uint32_t d = n;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const uint64_t a = __shfl_up(c, o, 64);
-    const uint32_t b = __shfl_up(d, o, 64);
-    if (lane >= o) c += a, d += b;
-  }
+  const uint64_t c = wave_scan_u64(w);
+  const uint32_t d = wave_scan_u32(n);
   __syncthreads();
   if (lane == 63) s.wpart[wave] = c, s.npart[wave] = d;
   __syncthreads();
@@ -684,10 +655,6 @@ __device__ __forceinline__ void draw_scan(DrawLds& s, uint64_t& w, uint32_t& n, 
   w = base + c - w, n = bn + d - n;
 }
 
-__device__ __forceinline__ uint64_t readlane_u64(uint64_t v, int lane) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
-}
 // A list entry: ~key in the upper half, its place in the vocabulary in the lower, so that rising entries are the order.
 __device__ __forceinline__ float entry_logit(uint64_t a) { return key_value(~(uint32_t)(a >> 32)); }
 
@@ -783,15 +750,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
       const uint64_t base = kind == kTopP ? in.before : 0;
       double want = 0;
       if (!by_count) {
-        uint64_t all = in.all;
-        if (kind == kTopK) {
-          uint64_t mine = 0;
-          uint32_t z = 0, zz;
-#pragma unroll
-          for (int q = 0; q < PER; q++) mine += sub[q] >= 0 && a[q] <= border ? f[q] : 0;
-          draw_scan(s, mine, z, all, zz);
-        }
-        want = r.top_p * (double)all;
+        want = r.top_p * (double)(kind == kTopK ? s.upto : in.all);
         // the border lies above what is listed, or below
         listed = (base == 0 || (double)base < want) && (double)(base + W) >= want;
         if (!listed) break;
@@ -815,7 +774,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
       if (tid < 64) {
         uint64_t c = s.base;
         uint32_t d = s.npart[0];
-        uint64_t at = ~0ull;
+        uint64_t at = ~0ull, upto = 0;
         for (int i0 = 0; i0 < m && at == ~0ull; i0 += 64) {  // 64 entries at a time: unsorted if there are no more
           const bool live = i0 + lane < m;
           const uint64_t x = live ? s.f.few[i0 + lane] : ~0ull;
@@ -831,9 +790,12 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
           const bool hit = live && (by_count ? rank == k - 1
                                              : ((double)before < want || before == 0) && (double)(before + w) >= want);
           const uint64_t who = __ballot(hit);
-          if (who) at = readlane_u64(x, __ffsll((long long)who) - 1);
+          if (who) {
+            const int j = __ffsll((long long)who) - 1;
+            at = readlane_u64(x, j), upto = readlane_u64(before + w, j);
+          }
         }
-        if (lane == 0) s.border = at;
+        if (lane == 0) s.border = at, s.upto = upto;
       }
       __syncthreads();
       border = s.border < border ? s.border : border;
@@ -897,11 +859,13 @@ size_t sample_workspace(int T, int V) { return (size_t)std::min(T, kRowsPerLaunc
 template <bool BF16>
 static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream_t st) {
   const auto blocks = [&](int waves) { return (ws.tiles + waves - 1) / waves; };
-  // a wave per tile where that does not fill the device; past it fewer blocks, which set up or join a histogram each
-  const dim3 some(std::min(blocks(kSomeWaves), std::max(1, 512 / a.T)), a.T), some_threads(64 * kSomeWaves);
+  // a wave per tile where that does not fill the device; past it fewer blocks, which set up or join a histogram each (128 rows
+  // of 248320: 512 / 768 / 1024 / 2048 blocks of k_sample_collect 122 / 116 / 118 / 122 us a call)
+  const auto some = [&](int most) { return dim3(std::min(blocks(kSomeWaves), std::max(1, most / a.T)), a.T); };
+  const dim3 some_threads(64 * kSomeWaves);
   hipLaunchKernelGGL(k_sample_max<BF16>, dim3(blocks(4), a.T), dim3(256), 0, st, a, ws);
-  if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some, some_threads, 0, st, a, ws);
-  hipLaunchKernelGGL(k_sample_collect<BF16>, some, some_threads, 0, st, a, ws);
+  if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some(512), some_threads, 0, st, a, ws);
+  hipLaunchKernelGGL(k_sample_collect<BF16>, some(kCollect), some_threads, 0, st, a, ws);
   hipLaunchKernelGGL(k_sample_draw<BF16>, dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
   return check_launch("sample");
 }
