@@ -6,8 +6,13 @@
 //   c_e = s_e + b_e; without a bias the logit itself, which has the order of its scores
 //   a group's value: its largest c, or the sum of its two largest (of s where there is no bias)
 //   picks: the k largest c among the topk_group best groups; weight s / sum of the picks' s, times a scale
-// Every choice is made in 64 bits, so that it is the formula's and not that of a rounding: in fp32 one token in some
-// thousands has two candidates a rounding apart.
+// Every choice is that of the formula in 64 bits, and not that of a rounding: in fp32 one token in some thousands has two
+// candidates a rounding apart.
+//
+// k_moe_route_fast decides in fp32 and looks at every gap that mattered: between a pick and the next one, the last one and
+// what was not picked, and between groups. Where one is within the error of the fp32 scores (one token in about a thousand)
+// the token's choice is made again in 64 bits by a whole wave, with the code of k_moe_route_ex. Without a bias the logits
+// themselves are compared, exactly.
 #include "common.h"
 #include "f64_dev.h"
 #include "host.h"
@@ -26,6 +31,12 @@ struct RouteExArgs {
   float* sg;
 };
 
+// LDS written by other lanes of this wave is read after it (a wave's LDS operations are in order: no instruction).
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Signed keys in the order of the values (64 bits; values are not NaN, -0 never enters).
 __device__ __forceinline__ int64_t key64(double v) {
   const int64_t u = __builtin_bit_cast(int64_t, v);
@@ -33,13 +44,11 @@ __device__ __forceinline__ int64_t key64(double v) {
 }
 constexpr int64_t kRouteGone = INT64_MIN;  // below every value's key: picked, cut off, or past E
 
-// One wave per token; lane l holds experts PER l .. + PER - 1 (PER = 1, 2, 4, 8 by E <= 512), so that a lane's logits are
+// One token by one wave; lane l holds experts PER l .. + PER - 1 (PER = 1, 2, 4, 8 by E <= 512), so that a lane's logits are
 // one load and a tie goes to the lowest lane.
 template <int PER, bool BF16, bool SOFTMAX, int GTOP>
-__global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
-  __shared__ double s_score[4][64 * PER];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x * 4 + wave;
-  if (t >= p.T) return;  // no block-wide barrier follows
+__device__ __forceinline__ void route_exact(const RouteExArgs& p, int t, double* score) {
+  const int lane = threadIdx.x & 63;
   const int e0 = lane * PER;
   float l[PER];
 #pragma unroll
@@ -74,7 +83,7 @@ __global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < PER; i++) s_score[wave][e0 + i] = s[i];
+  for (int i = 0; i < PER; i++) score[e0 + i] = s[i];
   int64_t key[PER];
   double c[PER];  // what the groups are ranked by
 #pragma unroll
@@ -136,10 +145,10 @@ __global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
         if (i == bi) key[i] = kRouteGone;
     }
   }
-  __builtin_amdgcn_wave_barrier();
+  wave_fence();
   // lane j < k <= 16: pick j
   const bool live = lane < p.k;
-  double v = live ? s_score[wave][who] : 0.0;
+  double v = live ? score[who] : 0.0;
   if (p.norm) {
     const double sum = dpp_sum_f64(v);
     v = sum > 0 ? v / sum : 0.0;
@@ -160,23 +169,287 @@ __global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
   }
 }
 
-template <int PER, bool BF16>
-static void launch_route_per(const RouteExArgs& a, int softmax, int group_top, hipStream_t st) {
-  const dim3 grid((a.T + 3) / 4), block(256);
-  if (softmax) {
-    if (group_top == 2) hipLaunchKernelGGL((k_moe_route_ex<PER, BF16, true, 2>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_moe_route_ex<PER, BF16, true, 1>), grid, block, 0, st, a);
-  } else {
-    if (group_top == 2) hipLaunchKernelGGL((k_moe_route_ex<PER, BF16, false, 2>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((k_moe_route_ex<PER, BF16, false, 1>), grid, block, 0, st, a);
+template <int PER, bool BF16, bool SOFTMAX, int GTOP>
+__global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
+  __shared__ double score[4][64 * PER];
+  const int wave = threadIdx.x >> 6, t = blockIdx.x * 4 + wave;
+  if (t < p.T) route_exact<PER, BF16, SOFTMAX, GTOP>(p, t, score[wave]);  // no block-wide barrier in it
+}
+
+// ---- several tokens per wave, in fp32 ------------------------------------------------------------------------------
+// LPR lanes per token (16 or 32), lane c of them holding experts PER c .. + PER - 1.
+
+// Reductions over a token's lanes, every lane getting the result: rotations by 8, 4, 2, 1 within 16 lanes, then the two rows
+// of 16 exchanged.
+template <int LPR, class Op>
+__device__ __forceinline__ uint32_t all_lanes(uint32_t v, Op op) {
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
+  v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
+  if constexpr (LPR == 32) {
+    const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(x[0], x[1]);
   }
+  return v;
+}
+template <int LPR>
+__device__ __forceinline__ uint32_t all_max(uint32_t v) {
+  return all_lanes<LPR>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+template <int LPR>
+__device__ __forceinline__ float all_max_f(float v) {
+  return __uint_as_float(all_lanes<LPR>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+template <int LPR>
+__device__ __forceinline__ float all_sum_f(float v) {
+  return __uint_as_float(all_lanes<LPR>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+// The sum over 16 lanes, in all of them.
+__device__ __forceinline__ double row_sum_f64(double v) {
+  v += dpp_f64<0x128, 0xf>(0.0, v);
+  v += dpp_f64<0x124, 0xf>(0.0, v);
+  v += dpp_f64<0x122, 0xf>(0.0, v);
+  return v + dpp_f64<0x121, 0xf>(0.0, v);
+}
+
+// PER values of a row from column col on, as they are (a lane that reaches past E: -infinity there).
+template <int PER, class T>
+__device__ __forceinline__ void load_run(const T* row, int col, int E, T pad, T (&v)[PER]) {
+  typedef T V __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
+  if (col + PER <= E) {
+    const V x = *(const V*)(row + col);
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = col + i < E ? row[min(col + i, E - 1)] : pad;
+  }
+}
+
+// Falling order of N values by Batcher's odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_falling(uint64_t (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; i++)
+          if (j + i + k < N && (j + i) / (2 * p) == (j + i + k) / (2 * p)) {
+            const uint64_t x = v[j + i], y = v[j + i + k];
+            const bool swap = x < y;
+            v[j + i] = swap ? y : x, v[j + i + k] = swap ? x : y;
+          }
+}
+
+// Whether two fp32 choices, or sums of two, may be in the other order. A sigmoid is off by less than 2^-22 (the exponential's
+// argument and its last place, the reciprocal's), a softmax by less than 2^-19 of itself (21 additions more), the bias's
+// addition and that of a group's two values by 2^-24 of their result. Equal infinities are exact.
+template <bool SOFTMAX>
+__device__ __forceinline__ bool too_near(float hi, float lo) {
+  const float m = __builtin_fmaf(fabsf(hi) + fabsf(lo), 0x1p-23f, SOFTMAX ? 0x1p-17f : 0x1p-20f);
+  return !(hi - lo > m) && !(hi == lo && fabsf(hi) == INFINITY);
+}
+
+template <int LPR, int PER, bool BF16, bool SOFTMAX, int GTOP>
+__global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
+  constexpr int RW = 64 / LPR;  // tokens per wave
+  // per wave: the tokens' choices (for the groups), then their lanes' sorted experts [PER][64], or a token's scores in 64 bits
+  __shared__ __align__(16) uint64_t mem[4][64 * PER];
+  __shared__ int s_pick[4][RW][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane / LPR, c = lane % LPR, e0 = c * PER;
+  const int t0 = (blockIdx.x * 4 + wave) * RW, t = t0 + r;
+  if (t0 >= p.T) return;  // no block-wide barrier follows
+  const size_t row = (size_t)min(t, p.T - 1) * p.stride;
+  float l[PER];
+  if constexpr (BF16) {
+    uint16_t h[PER];
+    load_run<PER, uint16_t>((const uint16_t*)p.logits + row, e0, p.E, 0xff80u, h);
+#pragma unroll
+    for (int i = 0; i < PER; i++) l[i] = bf2f(h[i]);
+  } else {
+    load_run<PER, float>((const float*)p.logits + row, e0, p.E, -INFINITY, l);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; i++) l[i] = fmaxf(l[i], -INFINITY) + 0.f;  // NaN: -infinity; -0: +0
+  const bool scores = p.bias != nullptr || (p.groups > 1 && GTOP == 2);
+  float mx = 0.f, s[PER];
+  if constexpr (SOFTMAX) {
+    mx = l[0];
+#pragma unroll
+    for (int i = 1; i < PER; i++) mx = fmaxf(mx, l[i]);
+    mx = all_max_f<LPR>(mx);
+  }
+  if (scores) {
+    if constexpr (SOFTMAX) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        s[i] = l[i] == mx ? 1.f : __builtin_amdgcn_exp2f((l[i] - mx) * 1.44269504f);
+        sum += e0 + i < p.E ? s[i] : 0.f;
+      }
+      const float rs = mx == -INFINITY ? 0.f : __builtin_amdgcn_rcpf(all_sum_f<LPR>(sum));
+#pragma unroll
+      for (int i = 0; i < PER; i++) s[i] *= rs;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; i++) s[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[i] * -1.44269504f));
+    }
+  }
+  // v: what is compared
+  float v[PER];
+  if (p.bias) {
+    load_run<PER, float>(p.bias, e0, p.E, -INFINITY, v);
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = s[i] + (fmaxf(v[i], -INFINITY) + 0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; i++) v[i] = l[i];
+  }
+  bool near = false;
+  uint32_t gone = 0;  // bit i: expert e0 + i is cut off
+  if (p.groups > 1) {
+    // every group by q = 2^n of the token's lanes, through LDS: whatever the groups' size
+    const int gs = p.E / p.groups, q = 1 << (31 - __builtin_clz(LPR / p.groups)), g = c / q, part = c % q;
+    float* const ch = (float*)mem[wave] + r * (LPR * PER);
+#pragma unroll
+    for (int i = 0; i < PER; i++) ch[e0 + i] = GTOP == 2 && !p.bias ? s[i] : v[i];
+    wave_fence();
+    float a = -INFINITY, b = -INFINITY;  // the two largest
+    if (g < p.groups)
+      for (int i = part; i < gs; i += q) {
+        const float x = ch[g * gs + i];
+        b = __builtin_amdgcn_fmed3f(a, b, x), a = fmaxf(a, x);
+      }
+    for (int o = 1; o < q; o *= 2) {
+      const float a2 = __shfl_xor(a, o, 64), b2 = __shfl_xor(b, o, 64);
+      b = fmaxf(fminf(a, a2), fmaxf(b, b2)), a = fmaxf(a, a2);
+    }
+    const float mine = GTOP == 1 ? a : b == -INFINITY ? b : a + b;
+    int rank = 0;
+    for (int o = 1; o < p.groups; o++) {
+      int og = g + o;
+      og -= og >= p.groups ? p.groups : 0;
+      const float x = __shfl(mine, r * LPR + min(og * q, LPR - 1), 64);
+      rank += x > mine || (x == mine && og < g);
+      if (p.bias || GTOP == 2) near |= g < p.groups && too_near<SOFTMAX>(fmaxf(x, mine), fminf(x, mine));
+    }
+    const uint64_t keep = __ballot(g < p.groups && rank < p.topk_groups) >> (r * LPR);
+    int eg = e0 / gs, left = gs - e0 % gs;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      gone |= (keep >> (min(eg, p.groups - 1) * q) & 1) ? 0u : 1u << i;
+      if (--left == 0) eg++, left = gs;
+    }
+    wave_fence();
+  }
+  uint64_t x[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++)
+    x[i] = e0 + i < p.E && !(gone >> i & 1) ? (uint64_t)order_key(v[i]) << 32 | (uint32_t)~(e0 + i) : 0ull;
+  sort_falling<PER>(x);
+  uint64_t* const sorted = mem[wave] + lane;
+#pragma unroll
+  for (int i = 1; i < PER; i++) sorted[64 * i] = x[i];
+  uint64_t head = x[0];
+  int next = 1;
+  float last = INFINITY;
+  for (int j = 0; j <= p.k; j++) {
+    const uint32_t hk = (uint32_t)(head >> 32), m = all_max<LPR>(hk);
+    bool win = hk == m;
+    const uint32_t same = (uint32_t)(__ballot(win) >> (r * LPR)) & (LPR == 32 ? 0xffffffffu : 0xffffu);
+    if (__ballot((same & (same - 1)) != 0)) {  // equal choices: the lowest expert
+      const uint32_t lo = win ? (uint32_t)head : 0u, low = all_max<LPR>(lo);  // (by all lanes)
+      win = win && lo == low;
+    }
+    if (p.bias) {
+      const float at = m ? key_value(m) : -INFINITY;  // m = 0: nothing is left
+      near |= j > 0 && m != 0 && too_near<SOFTMAX>(last, at);
+      last = at;
+    }
+    if (j == p.k) break;
+    if (win) {
+      s_pick[wave][r][j] = (int)~(uint32_t)head;
+      head = next < PER ? sorted[64 * next] : 0ull;
+      next++;
+    }
+  }
+  wave_fence();
+  // tokens with a near choice: again, in 64 bits
+  const uint64_t redo = __ballot(near && t < p.T);
+  auto redo_row = [&](int rr) { return (redo >> (rr * LPR) & (LPR == 32 ? 0xffffffffull : 0xffffull)) != 0; };
+  const int who = c < p.k ? s_pick[wave][r][c] : 0;
+  const bool live = c < p.k && t < p.T && !redo_row(r);
+  double w = 0;
+  if (c < p.k) {
+    const size_t o = row + who;
+    const double y = order_value(BF16 ? bf2f(((const uint16_t*)p.logits)[o]) : ((const float*)p.logits)[o]);
+    if constexpr (SOFTMAX) {
+      w = y == -INFINITY ? 0.0 : y == (double)mx ? 1.0 : exp_neg(y - (double)mx);
+    } else {
+      const double z = exp_neg(-fabs(y)), q = rcp64(1 + z);
+      w = y < 0 ? z * q : q;
+    }
+  }
+  double sum = 1.0;
+  if (p.norm) {
+    sum = row_sum_f64(w);
+  } else if constexpr (SOFTMAX) {
+    double all = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) all += l[i] == -INFINITY ? 0.0 : l[i] == mx ? 1.0 : exp_neg((double)l[i] - (double)mx);
+    sum = row_sum_f64(all);
+    if constexpr (LPR == 32) sum += __shfl_xor(sum, 16, 64);
+  }
+  w = sum > 0 ? w / sum : 0.0;
+  if (live) {
+    p.idx[(size_t)t * p.k + c] = who;
+    p.wt[(size_t)t * p.k + c] = (float)(w * (double)p.scale);
+  }
+  if (c == 0 && t < p.T && !redo_row(r)) {
+    float g = 1.f;
+    if (p.shared_gate) {
+      const double y = BF16 ? bf2f(((const uint16_t*)p.logits)[row + p.E]) : ((const float*)p.logits)[row + p.E];
+      const double z = exp_neg(-fabs(y));
+      g = (float)(y != y ? y : y < 0 ? z / (1 + z) : 1 / (1 + z));
+    }
+    p.sg[t] = g;
+  }
+  if (redo == 0) return;
+  for (int rr = 0; rr < RW; rr++)
+    if (redo_row(rr)) {
+      wave_fence();
+      route_exact<LPR * PER / 64, BF16, SOFTMAX, GTOP>(p, t0 + rr, (double*)mem[wave]);
+    }
+}
+
+// The lanes per token by E; groups of which a token has more than lanes go by waves.
+template <int LPR, int PER, bool BF16, bool SOFTMAX, int GTOP>
+static void launch_route_cfg(const RouteExArgs& a, hipStream_t st) {
+  constexpr int rows = 4 * 64 / LPR;
+  if (a.groups <= LPR)
+    hipLaunchKernelGGL((k_moe_route_fast<LPR, PER, BF16, SOFTMAX, GTOP>), dim3((a.T + rows - 1) / rows), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((k_moe_route_ex<LPR * PER / 64, BF16, SOFTMAX, GTOP>), dim3((a.T + 3) / 4), dim3(256), 0, st, a);
+}
+template <bool BF16, bool SOFTMAX, int GTOP>
+static void launch_route_e(const RouteExArgs& a, hipStream_t st) {
+  if (a.E <= 64) launch_route_cfg<16, 4, BF16, SOFTMAX, GTOP>(a, st);
+  else if (a.E <= 128) launch_route_cfg<16, 8, BF16, SOFTMAX, GTOP>(a, st);
+  else if (a.E <= 256) launch_route_cfg<16, 16, BF16, SOFTMAX, GTOP>(a, st);
+  else launch_route_cfg<32, 16, BF16, SOFTMAX, GTOP>(a, st);
 }
 template <bool BF16>
 static void launch_route_bf(const RouteExArgs& a, int softmax, int group_top, hipStream_t st) {
-  if (a.E <= 64) launch_route_per<1, BF16>(a, softmax, group_top, st);
-  else if (a.E <= 128) launch_route_per<2, BF16>(a, softmax, group_top, st);
-  else if (a.E <= 256) launch_route_per<4, BF16>(a, softmax, group_top, st);
-  else launch_route_per<8, BF16>(a, softmax, group_top, st);
+  if (softmax) group_top == 2 ? launch_route_e<BF16, true, 2>(a, st) : launch_route_e<BF16, true, 1>(a, st);
+  else group_top == 2 ? launch_route_e<BF16, false, 2>(a, st) : launch_route_e<BF16, false, 1>(a, st);
 }
 
 int launch_moe_route_ex(const void* logits, int logits_bf16, int T, int E, int k, int stride, int softmax,
