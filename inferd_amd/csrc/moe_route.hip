@@ -9,10 +9,10 @@
 // Every choice is that of the formula in 64 bits, and not that of a rounding: in fp32 one token in some thousands has two
 // candidates a rounding apart.
 //
-// k_moe_route_fast decides in fp32 and looks at every gap that mattered: between a pick and the next one, the last one and
-// what was not picked, and between groups. Where one is within the error of the fp32 scores (one token in about a thousand)
-// the token's choice is made again in 64 bits by a whole wave, with the code of k_moe_route_ex. Without a bias the logits
-// themselves are compared, exactly.
+// k_moe_route_fast takes the k + 1 largest in fp32, and where two neighbours among them are within the error of the fp32
+// scores (one token in some hundreds) orders them anew by their scores in 64 bits. Where that does not settle it (the next
+// one is as near to the last pick, or a group that stays to one that does not: one token in ten thousands) the token is done
+// again in 64 bits by a whole wave, with the code of k_moe_route_ex. Without a bias the logits themselves are compared.
 #include "common.h"
 #include "f64_dev.h"
 #include "host.h"
@@ -177,18 +177,22 @@ __global__ __launch_bounds__(256) void k_moe_route_ex(RouteExArgs p) {
 }
 
 // ---- several tokens per wave, in fp32 ------------------------------------------------------------------------------
-// LPR lanes per token (16 or 32), lane c of them holding experts PER c .. + PER - 1.
+// LPR lanes per token (16, 32 or 64), lane c of them holding experts PER c .. + PER - 1 (PER <= 16).
 
-// Reductions over a token's lanes, every lane getting the result: rotations by 8, 4, 2, 1 within 16 lanes, then the two rows
-// of 16 exchanged.
+// Reductions over a token's lanes, every lane getting the result: rotations by 8, 4, 2, 1 within 16 lanes, then rows of 16
+// and halves exchanged.
 template <int LPR, class Op>
 __device__ __forceinline__ uint32_t all_lanes(uint32_t v, Op op) {
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false));  // row_ror:8
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false));
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, false));
   v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, false));
-  if constexpr (LPR == 32) {
+  if constexpr (LPR >= 32) {
     const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(x[0], x[1]);
+  }
+  if constexpr (LPR == 64) {
+    const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = op(x[0], x[1]);
   }
   return v;
@@ -233,7 +237,7 @@ __device__ __forceinline__ void load_run(const T* row, int col, int E, T pad, T 
 
 // Falling order of N values by Batcher's odd-even merges.
 template <int N>
-__device__ __forceinline__ void sort_falling(uint64_t (&v)[N]) {
+__device__ __forceinline__ void sort_falling(uint32_t (&v)[N]) {
 #pragma unroll
   for (int p = 1; p < N; p *= 2)
 #pragma unroll
@@ -243,31 +247,39 @@ __device__ __forceinline__ void sort_falling(uint64_t (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < k; i++)
           if (j + i + k < N && (j + i) / (2 * p) == (j + i + k) / (2 * p)) {
-            const uint64_t x = v[j + i], y = v[j + i + k];
-            const bool swap = x < y;
-            v[j + i] = swap ? y : x, v[j + i + k] = swap ? x : y;
+            const uint32_t x = v[j + i], y = v[j + i + k];
+            v[j + i] = max(x, y), v[j + i + k] = min(x, y);
           }
 }
 
 // Whether two fp32 choices, or sums of two, may be in the other order. A sigmoid is off by less than 2^-22 (the exponential's
 // argument and its last place, the reciprocal's), a softmax by less than 2^-19 of itself (21 additions more), the bias's
-// addition and that of a group's two values by 2^-24 of their result. Equal infinities are exact.
-template <bool SOFTMAX>
+// addition and that of a group's two values by 2^-24 of their result; the last four bits of a key hide 2^-19 of a value.
+// Equal infinities are exact.
+template <bool SOFTMAX, bool KEYS>
 __device__ __forceinline__ bool too_near(float hi, float lo) {
-  const float m = __builtin_fmaf(fabsf(hi) + fabsf(lo), 0x1p-23f, SOFTMAX ? 0x1p-17f : 0x1p-20f);
+  const float m = __builtin_fmaf(fabsf(hi) + fabsf(lo), KEYS ? 0x1p-18f : 0x1p-23f, SOFTMAX ? 0x1p-17f : 0x1p-20f);
   return !(hi - lo > m) && !(hi == lo && fabsf(hi) == INFINITY);
 }
 
+// A lane's choices become 32-bit keys in the order of the values whose last four bits hold 15 - i, so that a sort takes two
+// instructions per exchange; the lanes' sorted keys lie in LDS, and each round takes the largest head by its upper 28 bits, the
+// lowest lane's where they are equal. That is exact for bf16 logits without a bias; else a gap that the four bits might hide
+// is a near one.
 template <int LPR, int PER, bool BF16, bool SOFTMAX, int GTOP>
 __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
+  static_assert(PER <= 16 && LPR >= 16, "four bits for a lane's experts, a lane for each of 16 picks");
   constexpr int RW = 64 / LPR;  // tokens per wave
-  // per wave: the tokens' choices (for the groups), then their lanes' sorted experts [PER][64], or a token's scores in 64 bits
+  constexpr uint64_t kLanes = LPR == 64 ? ~0ull : (1ull << (LPR % 64)) - 1;
+  // per wave: the tokens' choices (for the groups), then their lanes' sorted keys [PER][64], or a token's scores in 64 bits
   __shared__ __align__(16) uint64_t mem[4][64 * PER];
-  __shared__ int s_pick[4][RW][16];
+  __shared__ int s_pick[4][RW][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane / LPR, c = lane % LPR, e0 = c * PER;
   const int t0 = (blockIdx.x * 4 + wave) * RW, t = t0 + r;
   if (t0 >= p.T) return;  // no block-wide barrier follows
   const size_t row = (size_t)min(t, p.T - 1) * p.stride;
+  float bias[PER];
+  if (p.bias) load_run<PER, float>(p.bias, e0, p.E, -INFINITY, bias);
   float l[PER];
   if constexpr (BF16) {
     uint16_t h[PER];
@@ -306,14 +318,13 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
   // v: what is compared
   float v[PER];
   if (p.bias) {
-    load_run<PER, float>(p.bias, e0, p.E, -INFINITY, v);
 #pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = s[i] + (fmaxf(v[i], -INFINITY) + 0.f);
+    for (int i = 0; i < PER; i++) v[i] = s[i] + (fmaxf(bias[i], -INFINITY) + 0.f);
   } else {
 #pragma unroll
     for (int i = 0; i < PER; i++) v[i] = l[i];
   }
-  bool near = false;
+  bool redo_me = false;
   uint32_t gone = 0;  // bit i: expert e0 + i is cut off
   if (p.groups > 1) {
     // every group by q = 2^n of the token's lanes, through LDS: whatever the groups' size
@@ -323,23 +334,36 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
     for (int i = 0; i < PER; i++) ch[e0 + i] = GTOP == 2 && !p.bias ? s[i] : v[i];
     wave_fence();
     float a = -INFINITY, b = -INFINITY;  // the two largest
-    if (g < p.groups)
-      for (int i = part; i < gs; i += q) {
-        const float x = ch[g * gs + i];
-        b = __builtin_amdgcn_fmed3f(a, b, x), a = fmaxf(a, x);
+    for (int i0 = 0; i0 < gs; i0 += 8 * q) {  // eight reads in flight
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) x[u] = ch[min(g, p.groups - 1) * gs + min(i0 + q * u + part, gs - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        x[u] = i0 + q * u + part < gs ? x[u] : -INFINITY;
+        b = __builtin_amdgcn_fmed3f(a, b, x[u]), a = fmaxf(a, x[u]);
       }
+    }
     for (int o = 1; o < q; o *= 2) {
       const float a2 = __shfl_xor(a, o, 64), b2 = __shfl_xor(b, o, 64);
       b = fmaxf(fminf(a, a2), fmaxf(b, b2)), a = fmaxf(a, a2);
     }
     const float mine = GTOP == 1 ? a : b == -INFINITY ? b : a + b;
     int rank = 0;
-    for (int o = 1; o < p.groups; o++) {
-      int og = g + o;
-      og -= og >= p.groups ? p.groups : 0;
-      const float x = __shfl(mine, r * LPR + min(og * q, LPR - 1), 64);
-      rank += x > mine || (x == mine && og < g);
-      if (p.bias || GTOP == 2) near |= g < p.groups && too_near<SOFTMAX>(fmaxf(x, mine), fminf(x, mine));
+    for (int o0 = 0; o0 < p.groups; o0 += 4) {
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) x[u] = __shfl(mine, r * LPR + min((o0 + u) * q, LPR - 1), 64);
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int og = o0 + u;
+        const bool other = og < p.groups && og != g;
+        rank += other && (x[u] > mine || (x[u] == mine && og < g));
+      }
+    }
+    if (p.bias || GTOP == 2) {  // a group that stays against those that do not
+      const float out = all_max_f<LPR>(g < p.groups && rank >= p.topk_groups ? mine : -INFINITY);
+      redo_me = g < p.groups && rank < p.topk_groups && p.topk_groups < p.groups && too_near<SOFTMAX, false>(mine, out);
     }
     const uint64_t keep = __ballot(g < p.groups && rank < p.topk_groups) >> (r * LPR);
     int eg = e0 / gs, left = gs - e0 % gs;
@@ -350,47 +374,43 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
     }
     wave_fence();
   }
-  uint64_t x[PER];
+  uint32_t x[PER];  // 0: cut off, or past E (below every value's key)
 #pragma unroll
-  for (int i = 0; i < PER; i++)
-    x[i] = e0 + i < p.E && !(gone >> i & 1) ? (uint64_t)order_key(v[i]) << 32 | (uint32_t)~(e0 + i) : 0ull;
+  for (int i = 0; i < PER; i++) {
+    const uint32_t u = __float_as_uint(v[i]);
+    const uint32_t k = (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) & ~15u;
+    x[i] = e0 + i < p.E && !(gone >> i & 1) ? k | (15u - i) : 0u;
+  }
   sort_falling<PER>(x);
-  uint64_t* const sorted = mem[wave] + lane;
+  uint32_t* const sorted = (uint32_t*)mem[wave] + lane;
 #pragma unroll
   for (int i = 1; i < PER; i++) sorted[64 * i] = x[i];
-  uint64_t head = x[0];
+  wave_fence();
+  uint32_t head = x[0], picked = 0, m = 0, last = 0, rest = 0;  // keys: of the c-th largest, of the k-th, the one behind it
   int next = 1;
-  float last = INFINITY;
-  for (int j = 0; j <= p.k; j++) {
-    const uint32_t hk = (uint32_t)(head >> 32), m = all_max<LPR>(hk);
-    bool win = hk == m;
-    const uint32_t same = (uint32_t)(__ballot(win) >> (r * LPR)) & (LPR == 32 ? 0xffffffffu : 0xffffu);
-    if (__ballot((same & (same - 1)) != 0)) {  // equal choices: the lowest expert
-      const uint32_t lo = win ? (uint32_t)head : 0u, low = all_max<LPR>(lo);  // (by all lanes)
-      win = win && lo == low;
-    }
-    if (p.bias) {
-      const float at = m ? key_value(m) : -INFINITY;  // m = 0: nothing is left
-      near |= j > 0 && m != 0 && too_near<SOFTMAX>(last, at);
-      last = at;
-    }
-    if (j == p.k) break;
-    if (win) {
-      s_pick[wave][r][j] = (int)~(uint32_t)head;
-      head = next < PER ? sorted[64 * next] : 0ull;
+  const uint64_t below = ((1ull << c) - 1) << (r * LPR);
+  for (int j = 0; j <= p.k + 1; j++) {
+    const uint32_t hk = head & ~15u;
+    m = all_max<LPR>(hk);
+    if (j > p.k) break;
+    const bool best = hk == m;
+    const uint64_t same = __ballot(best);
+    picked = c == j ? m : picked;
+    last = j == p.k - 1 ? m : last, rest = m;
+    if (best && !(same & below)) {  // of equal choices the lowest lane's
+      s_pick[wave][r][j] = m ? e0 + 15 - (int)(head & 15u) : 0;  // (m = 0: nothing is left, j = k)
+      head = next < PER ? sorted[64 * next] : 0u;
       next++;
     }
   }
   wave_fence();
-  // tokens with a near choice: again, in 64 bits
-  const uint64_t redo = __ballot(near && t < p.T);
-  auto redo_row = [&](int rr) { return (redo >> (rr * LPR) & (LPR == 32 ? 0xffffffffull : 0xffffull)) != 0; };
-  const int who = c < p.k ? s_pick[wave][r][c] : 0;
-  const bool live = c < p.k && t < p.T && !redo_row(r);
-  double w = 0;
-  if (c < p.k) {
+  const int who = s_pick[wave][r][min(c, p.k)];
+  // the c-th score in 64 bits, and what is compared
+  const int few = min(p.k + 1, LPR);
+  double w = 0, y = 0;
+  if (c < few) {
     const size_t o = row + who;
-    const double y = order_value(BF16 ? bf2f(((const uint16_t*)p.logits)[o]) : ((const float*)p.logits)[o]);
+    y = order_value(BF16 ? bf2f(((const uint16_t*)p.logits)[o]) : ((const float*)p.logits)[o]);
     if constexpr (SOFTMAX) {
       w = y == -INFINITY ? 0.0 : y == (double)mx ? 1.0 : exp_neg(y - (double)mx);
     } else {
@@ -399,19 +419,44 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
     }
   }
   double sum = 1.0;
-  if (p.norm) {
-    sum = row_sum_f64(w);
-  } else if constexpr (SOFTMAX) {
-    double all = 0;
+  if constexpr (SOFTMAX)
+    if (p.bias || !p.norm) {
+      double all = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) all += l[i] == -INFINITY ? 0.0 : l[i] == mx ? 1.0 : exp_neg((double)l[i] - (double)mx);
-    sum = row_sum_f64(all);
-    if constexpr (LPR == 32) sum += __shfl_xor(sum, 16, 64);
+      for (int i = 0; i < PER; i++) all += l[i] == -INFINITY ? 0.0 : l[i] == mx ? 1.0 : exp_neg((double)l[i] - (double)mx);
+      sum = row_sum_f64(all);
+      if constexpr (LPR >= 32) sum += __shfl_xor(sum, 16, 64);
+      if constexpr (LPR == 64) sum += __shfl_xor(sum, 32, 64);
+      w = sum > 0 ? w / sum : 0.0;
+    }
+  int at = c;  // the place of this lane's expert among the few
+  if (p.bias || !BF16) {
+    const uint32_t after = (uint32_t)__shfl_down((int)picked, 1, 64);
+    const bool near = c + 1 < few && after != 0 && too_near<SOFTMAX, true>(key_value(picked), key_value(after));
+    // the one behind the few
+    const uint32_t beyond = few > p.k ? m : rest;
+    if (beyond != 0) redo_me |= too_near<SOFTMAX, true>(key_value(last), key_value(beyond));
+    if (__ballot(near)) {
+      const double mine = p.bias ? w + (double)order_value(p.bias[who]) : y;
+      at = 0;
+      for (int j = 0; j < few; j++) {
+        const double x = __shfl(mine, r * LPR + j, 64);
+        const int e = __shfl(who, r * LPR + j, 64);
+        at += __shfl((int)picked, r * LPR + j, 64) != 0 && (x > mine || (x == mine && e < who));
+      }
+    }
   }
-  w = sum > 0 ? w / sum : 0.0;
+  const uint64_t redo = __ballot(redo_me && t < p.T);
+  auto redo_row = [&](int rr) { return (redo >> (rr * LPR) & kLanes) != 0; };
+  const bool live = c < few && picked != 0 && at < p.k && t < p.T && !redo_row(r);
+  if (p.norm) {
+    sum = row_sum_f64(c < few && at < p.k ? w : 0.0);
+    if constexpr (LPR >= 32) sum += __shfl_xor(sum, 16, 64);  // the 17th lane's
+    w = sum > 0 ? w / sum : 0.0;
+  }
   if (live) {
-    p.idx[(size_t)t * p.k + c] = who;
-    p.wt[(size_t)t * p.k + c] = (float)(w * (double)p.scale);
+    p.idx[(size_t)t * p.k + at] = who;
+    p.wt[(size_t)t * p.k + at] = (float)(w * (double)p.scale);
   }
   if (c == 0 && t < p.T && !redo_row(r)) {
     float g = 1.f;
@@ -430,6 +475,12 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
     }
 }
 
+#ifndef R256
+#define R256 16, 16
+#endif
+#ifndef R512
+#define R512 32, 16
+#endif
 // The lanes per token by E; groups of which a token has more than lanes go by waves.
 template <int LPR, int PER, bool BF16, bool SOFTMAX, int GTOP>
 static void launch_route_cfg(const RouteExArgs& a, hipStream_t st) {
@@ -443,8 +494,8 @@ template <bool BF16, bool SOFTMAX, int GTOP>
 static void launch_route_e(const RouteExArgs& a, hipStream_t st) {
   if (a.E <= 64) launch_route_cfg<16, 4, BF16, SOFTMAX, GTOP>(a, st);
   else if (a.E <= 128) launch_route_cfg<16, 8, BF16, SOFTMAX, GTOP>(a, st);
-  else if (a.E <= 256) launch_route_cfg<16, 16, BF16, SOFTMAX, GTOP>(a, st);
-  else launch_route_cfg<32, 16, BF16, SOFTMAX, GTOP>(a, st);
+  else if (a.E <= 256) launch_route_cfg<R256, BF16, SOFTMAX, GTOP>(a, st);
+  else launch_route_cfg<R512, BF16, SOFTMAX, GTOP>(a, st);
 }
 template <bool BF16>
 static void launch_route_bf(const RouteExArgs& a, int softmax, int group_top, hipStream_t st) {
