@@ -433,15 +433,28 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p,
   int kind = row_kind(r, p.V, 0.f);
   if (kind != kTopP && !(kind == kTopK && blockIdx.x == 0)) return;
   for (int i = threadIdx.x; i < (kind == kTopK ? kTauBins : kBins); i += 64 * kSomeWaves) h[i] = 0;
+  // the first loads go out before the row's maximum is waited for
+  constexpr int T = 64 * kSomeWaves, U = 8;
+  const float* const rm = ws.rmax(t);
+  float l[16];
+  if (kind == kTopK) {
+#pragma unroll
+    for (int u = 0; u < U; u++) l[u] = rm[min(T * u + (int)threadIdx.x, ws.runs - 1)];
+  } else {
+    load_tile<BF16>(p, t, min((int)blockIdx.x * kSomeWaves + wave, ws.tiles - 1), l);
+  }
   const float mx = row_max<kSomeWaves>(ws, t, s);  // with a barrier
   if (row_kind(r, p.V, mx) != kind) return;
   if (kind == kTopK) {
     const float sc = bin_scale(r, kTauScale);
-    const float* const rm = ws.rmax(t);
-    for (int i = threadIdx.x; i < ws.runs; i += 64 * kSomeWaves) {
-      const float y = (mx - rm[i]) * sc;
+    auto count = [&](float m) {
+      const float y = (mx - m) * sc;
       if (y < (float)(kTauBins - 1)) atomicAdd(&h[(int)y], 1u);
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (T * u + (int)threadIdx.x < ws.runs) count(l[u]);
+    for (int i = T * U + threadIdx.x; i < ws.runs; i += T) count(rm[i]);
     __syncthreads();
     if (wave == 0) {  // the first bin at which k runs have been seen; without one, all that has a weight
       uint32_t n[16], own = 0;
@@ -462,8 +475,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p,
   }
   const float sc = bin_scale(r, kBinScale);
   for (int tile = blockIdx.x * kSomeWaves + wave; tile < ws.tiles; tile += kSomeWaves * gridDim.x) {
-    float l[16];
-    load_tile<BF16>(p, t, tile, l);
+    if (tile >= kSomeWaves * (int)gridDim.x) load_tile<BF16>(p, t, tile, l);
 #pragma unroll
     for (int e = 0; e < 16; e++) {
       const float y = (mx - l[e]) * sc;
@@ -530,6 +542,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
   const RowPar r = row_par(p, t);
   if (r.greedy) return;
+  const int tau = ws.info(t)->tau;
   const float mx = row_max<kSomeWaves>(ws, t, s);
   const int kind = row_kind(r, p.V, mx);
   if (kind != kTopK && kind != kTopP && kind != kFull) return;
@@ -539,7 +552,7 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p
   // y = (max - l) scale: below `sure` kept whole, from there to below `last` listed
   float sure = INFINITY, last = INFINITY, sc = 0.f;
   if (kind == kTopK) {
-    sure = 0.f, last = (float)(info->tau + 1), sc = bin_scale(r, kTauScale);
+    sure = 0.f, last = (float)(tau + 1), sc = bin_scale(r, kTauScale);
   } else if (kind == kTopP) {
     top_p_bins(ws.hist(t), r.top_p, part, bins);
     sure = (float)bins[0], last = (float)(bins[1] + 1), sc = bin_scale(r, kBinScale);
@@ -711,11 +724,12 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
 #pragma unroll
     for (int q = 0; q < PER; q++) {
       const int i = kRowThreads * q + tid;
-      if (q > 0 && kRowThreads * q < n) a[q] = ws.list(t)[min(i, n - 1)];
-      if (i >= n) a[q] = 0;
+      if (q > 0) a[q] = 0;
+      f[q] = 0;
+      if (kRowThreads * q >= n) continue;
+      if (q > 0) a[q] = ws.list(t)[min(i, n - 1)];
       const float l = entry_logit(a[q]);
-      f[q] = i < n ? weight(l, mx, r.rt) : 0;
-      if (i < n) lo = fminf(lo, l), hi = fmaxf(hi, l);
+      if (i < n) f[q] = weight(l, mx, r.rt), lo = fminf(lo, l), hi = fmaxf(hi, l);
     }
     lo = -dpp_max_f(-lo), hi = dpp_max_f(hi);
     if (lane == 0) s.npart[tid >> 6] = __float_as_uint(lo), s.s[tid >> 6] = hi;

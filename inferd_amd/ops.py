@@ -48,33 +48,37 @@ def _workspace_bytes(query: str, *sizes: int) -> int:
     return getattr(lib(), query)(*sizes)
 
 
-def _workspace_here(nbytes: int, device, stream: int):
+def _workspace_here(nbytes: int, device: int, stream: int):
     """The address of a zeroed workspace for one call on the current stream, and the tensor that holds it: cached per device
     and stream, and a fresh one inside a graph capture, so that calls on two streams, or two captured graphs, never share
     one."""
     if nbytes == 0:
         return None, None
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     else:
-        key = (device.index, stream)
-        buf = _ws_cache.get(key)
+        buf = _ws_cache.get((device, stream))
         if buf is None or buf.numel() < nbytes:
-            buf = _ws_cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            buf = _ws_cache[device, stream] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return buf.data_ptr(), buf
 
 
-def _check_tensors(device, **tensors) -> None:
-    """Each argument is (tensor or None, shape, dtype): of that shape and type, its rows' values adjacent, on `device`, which
-    is the current one (the calls go to its current stream)."""
-    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors on {device}, which is not the current device")
+def _differs(t: Optional[torch.Tensor], shape: tuple, dtype, device: int) -> bool:
+    """Whether an argument is there and not of this shape and type with a row's values adjacent on this device. (Each call
+    checks every argument: these are the cheapest ways to ask.)"""
+    return t is not None and (t.dtype is not dtype or t.get_device() != device or t.shape != shape
+                              or (t.stride(-1) != 1 and t.shape[-1] > 1))
+
+
+def _wanted(device: int, **tensors) -> ValueError:
+    """What is wrong with a call's arguments, each (tensor or None, shape, dtype)."""
+    if device < 0 or device != torch._C._cuda_getDevice():
+        return ValueError("the tensors are not on the current device, whose current stream the call goes to")
     for name, (t, shape, dtype) in tensors.items():
-        if t is None:
-            continue
-        if t.shape != shape or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and shape[-1] > 1):
-            raise ValueError(f"{name}: {tuple(shape)} {dtype} on {device} with adjacent values wanted, got "
-                             f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+        if _differs(t, shape, dtype, device):
+            return ValueError(f"{name}: {tuple(shape)} {dtype} on device {device} with adjacent values wanted, got "
+                              f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
+    return ValueError("bad arguments")
 
 
 @dataclass
@@ -243,20 +247,25 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 def _gemm_epi(name: str, A, W, bias, act, residual, C, fp32) -> torch.Tensor:
     if A.dim() != 2 or act not in ACTS:
         raise ValueError(f"A: a matrix wanted, act={act!r}: one of {sorted(ACTS)}")
-    (M, K), N, dev, bf16 = A.shape, W.N, A.device, torch.bfloat16
+    M, K = A.shape
+    N, dev, bf16 = W.N, A.get_device(), torch.bfloat16
     if C is None:
-        C = torch.empty((M, N), dtype=torch.float32 if fp32 else bf16, device=dev)
-    f32 = C.dtype == torch.float32
-    _check_tensors(dev, A=(A, (M, W.K), bf16), bias=(bias, (N,), bf16), residual=(residual, (M, N), bf16),
-                   C=(C, (M, N), C.dtype if f32 else bf16), weights=(W.wt, (W.wt.numel(),), torch.uint8))
+        C = torch.empty((M, N), dtype=torch.float32 if fp32 else bf16, device=A.device)
+    out = torch.float32 if C.dtype is torch.float32 else bf16
+    if (dev < 0 or dev != torch._C._cuda_getDevice() or _differs(A, (M, W.K), bf16, dev)
+            or _differs(C, (M, N), out, dev) or _differs(bias, (N,), bf16, dev) or _differs(residual, (M, N), bf16, dev)
+            or W.wt.get_device() != dev):
+        raise _wanted(dev, A=(A, (M, W.K), bf16), C=(C, (M, N), out), bias=(bias, (N,), bf16),
+                      residual=(residual, (M, N), bf16), weights=(W.wt, W.wt.shape, torch.uint8))
     need = _workspace_bytes(name + "_workspace", M, N, K)
     stream = _stream()
     ws, _keep = _workspace_here(need, dev, stream)
-    lda, ldc, ldr = A.stride(0), C.stride(0), 0 if residual is None else residual.stride(0)
     if M == 1:  # the stride of a single row says nothing
         lda, ldc, ldr = K, N, N
-    check(getattr(lib(), name)(_p(A), lda, _p(W.wt), N, K, _p(bias), ACTS[act], _p(residual), ldr, _p(C), ldc, M, f32, ws,
-                               need, stream))
+    else:
+        lda, ldc, ldr = A.stride(0), C.stride(0), 0 if residual is None else residual.stride(0)
+    check(getattr(lib(), name)(A.data_ptr(), lda, W.wt.data_ptr(), N, K, _p(bias), ACTS[act], _p(residual), ldr,
+                               C.data_ptr(), ldc, M, out is torch.float32, ws, need, stream))
     return C
 
 
@@ -286,20 +295,27 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
 
     temperature, top_p, min_p fp32 [T] and top_k int32 [T] hold a value per row; None is off for all rows
     (temperature 0: greedy; top_k 0, top_p 1, min_p 0: off for that row). See ifd_sample for the rule."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+    f32, i32 = torch.float32, torch.int32
+    if logits.dim() != 2 or logits.dtype not in (f32, torch.bfloat16):
         raise ValueError(f"logits: a matrix of fp32 or bf16 wanted, got {tuple(logits.shape)} {logits.dtype}")
-    (T, V), dev, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
-    token, prob = outs if outs is not None else (torch.empty((T,), dtype=i32, device=dev),
-                                                 torch.empty((T,), dtype=f32, device=dev))
-    row = (T,)
-    _check_tensors(dev, logits=(logits, (T, V), logits.dtype), u=(u, row, f32), temperature=(temperature, row, f32),
-                   top_k=(top_k, row, i32), top_p=(top_p, row, f32), min_p=(min_p, row, f32), token=(token, row, i32),
-                   prob=(prob, row, f32))
+    T, V = logits.shape
+    dev, row = logits.get_device(), (T,)
+    if outs is None:
+        outs = (torch.empty(row, dtype=i32, device=logits.device), torch.empty(row, dtype=f32, device=logits.device))
+    token, prob = outs
+    if (dev < 0 or dev != torch._C._cuda_getDevice() or _differs(logits, (T, V), logits.dtype, dev)
+            or _differs(u, row, f32, dev) or _differs(temperature, row, f32, dev) or _differs(top_k, row, i32, dev)
+            or _differs(top_p, row, f32, dev) or _differs(min_p, row, f32, dev) or _differs(token, row, i32, dev)
+            or _differs(prob, row, f32, dev)):
+        raise _wanted(dev, logits=(logits, (T, V), logits.dtype), u=(u, row, f32), temperature=(temperature, row, f32),
+                      top_k=(top_k, row, i32), top_p=(top_p, row, f32), min_p=(min_p, row, f32), token=(token, row, i32),
+                      prob=(prob, row, f32))
     need = _workspace_bytes("ifd_sample_workspace", T, V)
     stream = _stream()
     ws, _keep = _workspace_here(need, dev, stream)
-    check(lib().ifd_sample(_p(logits), logits.dtype == torch.bfloat16, T, V, logits.stride(0) if T > 1 else V,
-                           _p(temperature), _p(top_k), _p(top_p), _p(min_p), _p(u), _p(token), _p(prob), ws, need, stream))
+    check(lib().ifd_sample(logits.data_ptr(), logits.dtype is torch.bfloat16, T, V, logits.stride(0) if T > 1 else V,
+                           _p(temperature), _p(top_k), _p(top_p), _p(min_p), u.data_ptr(), token.data_ptr(),
+                           prob.data_ptr(), ws, need, stream))
     return token, prob
 
 
@@ -443,21 +459,28 @@ def moe_route_ex(logits: torch.Tensor, E: int, k: int, score: str = "softmax", b
     topk_groups best stay, weights renormalised (norm) and scaled; see ifd_moe_route_ex for the rule. logits [T, >= E (+ 1
     with shared_gate)] fp32 or bf16. Returns (idx int32 [T, k], wt fp32 [T, k], sg fp32 [T]), as moe_route, written to
     `outs` when given."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or score not in SCORES:
+    f32, i32 = torch.float32, torch.int32
+    if logits.dim() != 2 or logits.dtype not in (f32, torch.bfloat16) or score not in SCORES:
         raise ValueError(f"logits: a matrix of fp32 or bf16 wanted, score={score!r}: one of {sorted(SCORES)}")
-    (T, width), dev, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
+    T, width = logits.shape
     if width < E + (1 if shared_gate else 0):
         raise ValueError(f"logits: {width} columns for E={E} (+ shared gate)")
-    idx, wt, sg = outs if outs is not None else (torch.empty((T, k), dtype=i32, device=dev),
-                                                 torch.empty((T, k), dtype=f32, device=dev),
-                                                 torch.empty((T,), dtype=f32, device=dev))
-    _check_tensors(dev, logits=(logits, (T, width), logits.dtype), bias=(bias, (E,), f32), idx=(idx, (T, k), i32),
-                   wt=(wt, (T, k), f32), sg=(sg, (T,), f32))
+    dev = logits.get_device()
+    if outs is None:
+        outs = (torch.empty((T, k), dtype=i32, device=logits.device), torch.empty((T, k), dtype=f32, device=logits.device),
+                torch.empty((T,), dtype=f32, device=logits.device))
+    idx, wt, sg = outs
+    if (dev < 0 or dev != torch._C._cuda_getDevice() or _differs(logits, (T, width), logits.dtype, dev)
+            or _differs(bias, (E,), f32, dev) or _differs(idx, (T, k), i32, dev) or _differs(wt, (T, k), f32, dev)
+            or _differs(sg, (T,), f32, dev)):
+        raise _wanted(dev, logits=(logits, (T, width), logits.dtype), bias=(bias, (E,), f32), idx=(idx, (T, k), i32),
+                      wt=(wt, (T, k), f32), sg=(sg, (T,), f32))
     if not (idx.is_contiguous() and wt.is_contiguous()):
         raise ValueError("idx and wt must be contiguous")
-    check(lib().ifd_moe_route_ex(_p(logits), logits.dtype == torch.bfloat16, T, E, k, logits.stride(0) if T > 1 else width,
-                                 SCORES[score], _p(bias), groups, topk_groups, group_top, norm, scale, shared_gate, _p(idx),
-                                 _p(wt), _p(sg), _stream()))
+    check(lib().ifd_moe_route_ex(logits.data_ptr(), logits.dtype is torch.bfloat16, T, E, k,
+                                 logits.stride(0) if T > 1 else width, SCORES[score], _p(bias), groups, topk_groups,
+                                 group_top, norm, scale, shared_gate, idx.data_ptr(), wt.data_ptr(), sg.data_ptr(),
+                                 _stream()))
     return idx, wt, sg
 
 
