@@ -430,3 +430,192 @@ def test_epilogue_infinities_and_nan(M):
         ref = _act64(A.double() @ _weights_as_used(w, M, N, K, 4).T.contiguous() + bias.double(), act) + R.double()
         assert torch.equal(out.isnan(), ref.isnan()), act
         assert torch.equal(out == math.inf, ref == math.inf) and torch.equal(out == -math.inf, ref == -math.inf), act
+
+
+# ---- empty calls, streams, graphs, and the run of a decode step --------------------------------------------------------
+def test_calls_without_rows():
+    ops = _ops()
+    W, _ = _layer(64, 256, 4, 1)
+    z = lambda *s, **k: torch.zeros(s, device="cuda", **k)  # noqa: E731
+    assert ops.gemm_t64_epi(z(0, 256, dtype=torch.bfloat16), W, act="relu").shape == (0, 64)
+    token, prob = ops.sample(z(0, 1000), z(0))
+    assert token.shape == prob.shape == (0,)
+    idx, wt, sg = ops.moe_route_ex(z(0, 64), 64, 4)
+    assert idx.shape == wt.shape == (0, 4) and sg.shape == (0,)
+
+
+def _step(T=6, seed=0):
+    """The layers and buffers of a small decode step: a projection with bias into the residual stream, experts routed by
+    sigmoid scores in groups, a head and its sampling."""
+    g, ops = _gu(), _ops()
+    H, I, E, k, V = 512, 64, 32, 4, 2000
+    gt = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=gt)  # noqa: E731
+
+    def scaled(N, K, s):  # products of about the inputs' size
+        codes, wq, sc, b = gen.qlinear(N, K, seed=s)
+        f = np.float32(1 / (0.0125 * 4.6 * math.sqrt(K)))
+        sc = gen.f32_to_bf16(gen.bf16_to_f32(sc) * f)
+        b = gen.f32_to_bf16(-7.5 * gen.bf16_to_f32(sc))
+        return codes, wq, sc, b
+
+    def stack(N, K, s):
+        parts = [scaled(N, K, s + e) for e in range(E)]
+        wq, sc, b = (np.stack([q[i] for q in parts]) for i in (1, 2, 3))
+        dense = torch.from_numpy(np.stack([gen.dequant_f64(q[0], q[2], q[3]) for q in parts])).cuda()
+        return ops.pack_t64_stack(g.moew(wq, sc, b)), dense
+
+    def linear(N, K, s):
+        codes, wq, sc, b = scaled(N, K, s)
+        return ops.pack_t64(g.qlinear(wq, sc, b)), torch.from_numpy(gen.dequant_f64(codes, sc, b)).cuda()
+
+    d = dict(H=H, I=I, E=E, k=k, V=V, T=T, proj=linear(H, H, 1), egu=stack(2 * I, H, 100), edn=stack(H, I, 200),
+             head=linear(V, H, 2), bias=rnd(H).to(torch.bfloat16), nw=(1 + 0.1 * rnd(H)).to(torch.bfloat16),
+             router=(rnd(E, H) * H ** -0.5).to(torch.bfloat16), balance=0.1 * rnd(E),
+             temperature=_col(T, [0.8, 0.0, 1.2]), top_k=_col(T, [50, 0, 5], torch.int32), top_p=_col(T, [0.9, 1.0]),
+             min_p=_col(T, [0.0, 0.02]))
+    return d
+
+
+def _run_step(d, a, x, u):
+    """The calls of the step: attention output a and residual stream x bf16 [T, H]; returns what each leaves."""
+    ops = _ops()
+    x1 = ops.gemm_t64_epi(a, d["proj"][0], bias=d["bias"], residual=x)
+    xn = ops.rmsnorm(x1, d["nw"], 1e-6)
+    logits = ops.moe_router_logits(xn, d["router"], out_bf16=False)
+    idx, wt, sg = ops.moe_route_ex(logits, d["E"], d["k"], score="sigmoid", bias=d["balance"], groups=4, topk_groups=2,
+                                   group_top=2, scale=2.5)
+    x2 = ops.moe_rows_t64(xn, idx, wt, None, d["egu"][0], d["edn"][0], out=x1.clone(), assign=False)
+    hn = ops.rmsnorm(x2, d["nw"], 1e-6)
+    head = ops.gemm_t64(hn, d["head"][0], mode=2)
+    token, prob = ops.sample(head, u, temperature=d["temperature"], top_k=d["top_k"], top_p=d["top_p"], min_p=d["min_p"])
+    return dict(x1=x1, xn=xn, logits=logits, idx=idx, wt=wt, sg=sg, x2=x2, hn=hn, head=head, token=token, prob=prob)
+
+
+def _step_inputs(d, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
+    return rnd(d["T"], d["H"]), rnd(d["T"], d["H"]), torch.rand((d["T"],), device="cuda", generator=g)
+
+
+def test_decode_step():
+    """The operators in a run, each against its 64-bit plain form on what the one before it left."""
+    d = _step()
+    a, x, u = _step_inputs(d, 1)
+    r = _run_step(d, a, x, u)
+    K, h = d["H"], 2.0 ** -8
+    y = a.double() @ d["proj"][1].T.contiguous() + d["bias"].double() + x.double()
+    tol = (K + 16) * 2.0 ** -24 * (a.double().abs() @ d["proj"][1].abs().T.contiguous())
+    assert bool(((r["x1"].double() - y).abs() <= h * (y.abs() + tol) + tol).all())
+    idx, wt, _ = plain_route(r["logits"], d["E"], d["k"], "sigmoid", d["balance"], 4, 2, 2, True, 2.5, False)
+    assert np.array_equal(r["idx"].cpu().numpy(), idx)
+    assert np.all(np.abs(r["wt"].cpu().numpy() - wt) <= 2.0 ** -24 * (1 + 1e-6) * wt)
+    # the experts' products on that routing: gate and up, their SwiGLU (three roundings to bf16), down, the weighted sum
+    xn, gu, dn = r["xn"].double(), d["egu"][1], d["edn"][1]
+    out, slack = torch.zeros_like(xn), torch.zeros_like(xn)
+    for t in range(d["T"]):
+        for j in range(d["k"]):
+            e, w = int(r["idx"][t, j]), float(r["wt"][t, j])
+            v = gu[e] @ xn[t]
+            gate, up = v[:d["I"]], v[d["I"]:]
+            hid = gate * torch.sigmoid(gate) * up
+            # d(hid): gate and up off by a rounding each (slope of x sigmoid(x) at most 1.1), then two more roundings
+            off = h * (1.1 * gate.abs() * up.abs() + 3 * hid.abs()) * 1.1
+            out[t] += w * (dn[e] @ hid)
+            slack[t] += w * (dn[e].abs() @ off)
+    ref = r["x1"].double() + out
+    # the sum is rounded before it is added, and the result is
+    assert bool(((r["x2"].double() - ref).abs() <= 1.01 * slack + 1.01 * h * (out.abs() + ref.abs()) + 1e-3 * slack).all())
+    token, prob = plain_sample(r["head"], u, d["temperature"], d["top_k"], d["top_p"], d["min_p"])
+    assert np.array_equal(r["token"].cpu().numpy(), token)
+    assert np.allclose(r["prob"].cpu().numpy(), prob, rtol=2.0 ** -23, atol=0)
+
+
+def test_routing_feeds_the_sorted_experts():
+    """moe_route_ex -> moe_dispatch: the expert-sorted rows, and the experts' products over them."""
+    ops = _ops()
+    d = _step(T=40, seed=3)
+    _, x, _ = _step_inputs(d, 4)
+    logits = ops.moe_router_logits(x, d["router"], out_bf16=False)
+    idx, wt, sg = ops.moe_route_ex(logits, d["E"], d["k"], score="sigmoid", bias=d["balance"], groups=8, topk_groups=3)
+    rows = ops.moe_rows_t64(x, idx, wt, None, d["egu"][0], d["edn"][0])
+    offsets, perm, inv, *_ = ops.moe_dispatch(idx, d["E"])
+    e = idx.flatten()[perm.long()]
+    assert bool((e[1:] >= e[:-1]).all()) and int(offsets[-1]) == idx.numel()
+    out = torch.zeros_like(rows, dtype=torch.float64)
+    for q in range(perm.numel()):
+        t, j = divmod(int(perm[q]), d["k"])
+        v = d["egu"][1][int(idx[t, j])] @ x[t].double()
+        hid = v[:d["I"]] * torch.sigmoid(v[:d["I"]]) * v[d["I"]:]
+        out[t] += float(wt[t, j]) * (d["edn"][1][int(idx[t, j])] @ hid)
+    assert float((rows.double() - out).norm() / out.norm()) < 2.0 ** -7  # a few roundings to bf16 of half a step each
+
+
+def test_streams_have_their_own_workspaces():
+    """The same calls on two streams at once, over and over: each gets the results it gets alone."""
+    d = _step(T=9)
+    ins = [_step_inputs(d, s) for s in (5, 6)]
+    alone = [_run_step(d, *i) for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    for _ in range(5):
+        got = []
+        for s, i in zip(streams, ins):
+            with torch.cuda.stream(s):
+                got.append(_run_step(d, *i))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            for name in a:
+                assert torch.equal(a[name], b[name]), name
+
+
+def test_two_captured_graphs():
+    """Two graphs of the step, replayed with new inputs, eager calls and synchronizations between; every replay gives the
+    eager result."""
+    d = _step(T=5)
+    eager = {s: _run_step(d, *_step_inputs(d, s)) for s in (7, 8, 9)}
+    graphs = []
+    for _ in range(2):
+        ins = _step_inputs(d, 7)
+        _run_step(d, *ins)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = _run_step(d, *ins)
+        graphs.append((graph, ins, outs))
+    for round_, s in enumerate((8, 9, 7, 8, 8, 9)):
+        for k, (graph, ins, outs) in enumerate(graphs):
+            for buf, new in zip(ins, _step_inputs(d, s)):
+                buf.copy_(new)
+            graph.replay()
+            if round_ % 2:
+                _run_step(d, *_step_inputs(d, 7))
+            if round_ % 3 == 0:
+                torch.cuda.synchronize()
+            for name in outs:
+                assert torch.equal(outs[name], eager[s][name]), (round_, k, name)
+
+
+def test_results_do_not_depend_on_the_batch_or_the_call():
+    """A row alone, in a batch, and again: the same token and routing (sums that atomics order would show here)."""
+    ops = _ops()
+    l, u, _ = _lm_logits(33, 30000, 21)
+    kw = dict(temperature=_col(33, [1.1]), top_p=_col(33, [0.93]), min_p=_col(33, [0.001]))
+    first = ops.sample(l, u, **kw)
+    for _ in range(5):
+        again = ops.sample(l, u, **kw)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    for r in (0, 7, 32):
+        one = ops.sample(l[r:r + 1], u[r:r + 1], **{n: t[r:r + 1] for n, t in kw.items()})
+        assert torch.equal(one[0][0], first[0][r]) and torch.equal(one[1][0], first[1][r])
+    q = torch.randn((65, 256), device="cuda")
+    whole = ops.moe_route_ex(q, 256, 8, score="sigmoid", groups=8, topk_groups=4, group_top=2)
+    for r in (0, 13, 64):
+        one = ops.moe_route_ex(q[r:r + 1], 256, 8, score="sigmoid", groups=8, topk_groups=4, group_top=2)
+        assert all(torch.equal(a[0], b[r]) for a, b in zip(one, whole))
+
+
+def test_sample_past_one_launch_of_rows():
+    """More rows than one set of launches takes."""
+    l, u, _ = _lm_logits(1100, 700, 31, bf16=True)
+    check_sample(l, u, top_k=_col(1100, [0, 20], torch.int32), top_p=_col(1100, [0.9, 1.0, 0.5]))
