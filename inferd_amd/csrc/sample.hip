@@ -294,8 +294,8 @@ __device__ __attribute__((noinline)) void row_sample(RowLds& s, const SampleArgs
 // The estimate only chooses what is listed: k_sample_draw checks that the exact border lies inside. Where it does not, or
 // the list is full (thousands of equal logits at the border, top_p within 4e-4 of 1 on a flat row), top_k is past 1024 or
 // the maximum infinite, it takes the one-block path above. Both give the same token.
-constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 4096, kTauBins = 1024;
-constexpr float kBinScale = 128.f, kTauScale = 32.f;  // bins per unit of (max - l) / temperature
+constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 4096;
+constexpr float kBinScale = 128.f;  // bins per unit of (max - l) / temperature
 constexpr int kRowsPerLaunch = 512, kSomeWaves = 8, kCollect = 768;
 
 struct RowInfo {  // what the launches of a call hand on, per row
@@ -425,14 +425,14 @@ __device__ __forceinline__ float bin_scale(const RowPar& r, float scale) {
 
 template <bool BF16>
 __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p, SampleWs ws) {
-  __shared__ uint32_t h[kBins];
+  __shared__ uint32_t h[kBins], part[kSomeWaves];
   __shared__ float s[kSomeWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
   const RowPar r = row_par(p, t);
   // (a maximum above -infinity and below infinity: whether it is that comes after the rows that have no work here)
   int kind = row_kind(r, p.V, 0.f);
   if (kind != kTopP && !(kind == kTopK && blockIdx.x == 0)) return;
-  for (int i = threadIdx.x; i < (kind == kTopK ? kTauBins : kBins); i += 64 * kSomeWaves) h[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += 64 * kSomeWaves) h[i] = 0;
   // the first loads go out before the row's maximum is waited for
   constexpr int T = 64 * kSomeWaves, U = 8;
   const float* const rm = ws.rmax(t);
@@ -445,35 +445,40 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_border(SampleArgs p,
   }
   const float mx = row_max<kSomeWaves>(ws, t, s);  // with a barrier
   if (row_kind(r, p.V, mx) != kind) return;
+  const float sc = bin_scale(r, kBinScale);
   if (kind == kTopK) {
-    const float sc = bin_scale(r, kTauScale);
     auto count = [&](float m) {
       const float y = (mx - m) * sc;
-      if (y < (float)(kTauBins - 1)) atomicAdd(&h[(int)y], 1u);
+      if (y < (float)(kBins - 1)) atomicAdd(&h[(int)y], 1u);
     };
 #pragma unroll
     for (int u = 0; u < U; u++)
       if (T * u + (int)threadIdx.x < ws.runs) count(l[u]);
     for (int i = T * U + threadIdx.x; i < ws.runs; i += T) count(rm[i]);
     __syncthreads();
-    if (wave == 0) {  // the first bin at which k runs have been seen; without one, all that has a weight
-      uint32_t n[16], own = 0;
+    // the first bin at which k runs have been seen; without one, all that has a weight
+    constexpr int PER = kBins / T;
+    uint32_t n[PER], own = 0;
 #pragma unroll
-      for (int i = 0; i < 16; i++) own += n[i] = h[16 * lane + i];
-      const uint32_t c = wave_scan_u32(own);
-      const uint64_t hit = __ballot(c >= (uint32_t)r.k);
-      if (hit == 0) {
-        if (lane == 0) ws.info(t)->tau = kTauBins - 2;
-      } else if (lane == __ffsll((long long)hit) - 1) {
-        uint32_t x = c - own;
-        int b = 0;
-        for (; b < 15 && x + n[b] < (uint32_t)r.k; b++) x += n[b];
-        ws.info(t)->tau = min(16 * lane + b, kTauBins - 2);
-      }
+    for (int i = 0; i < PER; i++) own += n[i] = h[PER * threadIdx.x + i];
+    const uint32_t c = wave_scan_u32(own);
+    if (lane == 63) part[wave] = c;
+    __syncthreads();
+    uint32_t x = c - own, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSomeWaves; i++) {
+      x += i < wave ? part[i] : 0;
+      all += part[i];
+    }
+    const uint32_t k = (uint32_t)r.k;
+    if (threadIdx.x == 0 && all < k) ws.info(t)->tau = kBins - 2;
+    if (x < k && x + own >= k) {
+      int b = 0;
+      for (; b < PER - 1 && x + n[b] < k; b++) x += n[b];
+      ws.info(t)->tau = min(PER * (int)threadIdx.x + b, kBins - 2);
     }
     return;
   }
-  const float sc = bin_scale(r, kBinScale);
   for (int tile = blockIdx.x * kSomeWaves + wave; tile < ws.tiles; tile += kSomeWaves * gridDim.x) {
     if (tile >= kSomeWaves * (int)gridDim.x) load_tile<BF16>(p, t, tile, l);
 #pragma unroll
@@ -550,12 +555,13 @@ __global__ __launch_bounds__(64 * kSomeWaves) void k_sample_collect(SampleArgs p
   if (threadIdx.x == 0) nfound = 0;
   __syncthreads();
   // y = (max - l) scale: below `sure` kept whole, from there to below `last` listed
-  float sure = INFINITY, last = INFINITY, sc = 0.f;
+  float sure = INFINITY, last = INFINITY;
+  const float sc = bin_scale(r, kBinScale);
   if (kind == kTopK) {
-    sure = 0.f, last = (float)(tau + 1), sc = bin_scale(r, kTauScale);
+    sure = 0.f, last = (float)(tau + 1);
   } else if (kind == kTopP) {
     top_p_bins(ws.hist(t), r.top_p, part, bins);
-    sure = (float)bins[0], last = (float)(bins[1] + 1), sc = bin_scale(r, kBinScale);
+    sure = (float)bins[0], last = (float)(bins[1] + 1);
   }
   auto add_to_list = [&](int tile, const float (&l)[16], const float (&y)[16]) {
 #pragma unroll
@@ -671,6 +677,45 @@ __device__ __forceinline__ void draw_scan(DrawLds& s, uint64_t& w, uint32_t& n, 
 // A list entry: ~key in the upper half, its place in the vocabulary in the lower, so that rising entries are the order.
 __device__ __forceinline__ float entry_logit(uint64_t a) { return key_value(~(uint32_t)(a >> 32)); }
 
+// The value of the lane whose number differs in bit M.
+template <int M>
+__device__ __forceinline__ uint32_t xor_lane(uint32_t v) {
+  if constexpr (M == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);  // quad_perm 1 0 3 2
+  else if constexpr (M == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);  // 2 3 0 1
+  else if constexpr (M == 4) return (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x101F);  // xor 4
+  else if constexpr (M == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false);  // row_ror:8
+  else if constexpr (M == 16) {
+    const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? x[0] : x[1];
+  } else {
+    const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? x[0] : x[1];
+  }
+}
+// One exchange of a bitonic sort over a wave: runs of K lanes rise and fall in turn; w goes along with v.
+template <int K, int M>
+__device__ __forceinline__ void exchange(uint64_t& v, uint64_t& w) {
+  const u32x2 a = __builtin_bit_cast(u32x2, v), b = __builtin_bit_cast(u32x2, w);
+  const uint64_t x = __builtin_bit_cast(uint64_t, u32x2{xor_lane<M>(a[0]), xor_lane<M>(a[1])});
+  const uint64_t y = __builtin_bit_cast(uint64_t, u32x2{xor_lane<M>(b[0]), xor_lane<M>(b[1])});
+  const bool low = ((threadIdx.x & M) == 0) == ((threadIdx.x & K) == 0);  // this lane keeps the smaller
+  if (low ? x < v : x > v) v = x, w = y;
+}
+template <int K, int M>
+__device__ __forceinline__ void merge_lanes(uint64_t& v, uint64_t& w) {
+  exchange<K, M>(v, w);
+  if constexpr (M > 1) merge_lanes<K, M / 2>(v, w);
+}
+// Sorts v over the 64 lanes, rising, w going along.
+__device__ __forceinline__ void sort_lanes(uint64_t& v, uint64_t& w) {
+  merge_lanes<2, 1>(v, w);
+  merge_lanes<4, 2>(v, w);
+  merge_lanes<8, 4>(v, w);
+  merge_lanes<16, 8>(v, w);
+  merge_lanes<32, 16>(v, w);
+  merge_lanes<64, 32>(v, w);
+}
+
 template <bool BF16>
 __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, SampleWs ws) {
   __shared__ DrawLds s;
@@ -714,6 +759,22 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
     return;
   }
   const int n = (int)min(in.n, (uint32_t)kList + 1);
+  if (kind == kTopK && n <= 64) {  // a short list by one wave: sorted, cut, and sorted again into the vocabulary's order
+    if (tid >= 64) return;
+    uint64_t e = lane < n ? a[0] : ~0ull, w = lane < n ? weight(entry_logit(a[0]), mx, r.rt) : 0;
+    sort_lanes(e, w);
+    if (lane >= r.k) w = 0;
+    const uint64_t upto = wave_scan_u64(w);
+    const double part = r.top_p * (double)readlane_u64(upto, 63);
+    if (r.top_p < 1.0 && lane > 0 && !((double)(upto - w) < part)) w = 0;
+    if (w < r.min_w) w = 0;
+    uint64_t place = e << 32 | (uint32_t)lane;
+    sort_lanes(place, w);
+    const uint64_t sum = wave_scan_u64(w), total = readlane_u64(sum, 63);
+    const uint64_t hit = __ballot(w != 0 && (double)sum > u * (double)total);
+    if (hit && lane == __ffsll((long long)hit) - 1) done((int)(place >> 32), (float)((double)w / (double)total));
+    return;
+  }
   bool listed = kind != kOneBlock && n <= kList;
   // what is kept: the prefix of the order up to the entry `border`, as far as it has min_p
   uint64_t border = ~0ull;
