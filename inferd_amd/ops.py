@@ -11,6 +11,7 @@ from typing import Optional
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -49,17 +50,18 @@ def _workspace_bytes(query: str, *sizes: int) -> int:
 
 
 def _workspace_here(nbytes: int, device: int, stream: int):
-    """The address of a zeroed workspace for one call on the current stream, and the tensor that holds it: cached per device
-    and stream, and a fresh one inside a graph capture, so that calls on two streams, or two captured graphs, never share
-    one."""
+    """The address of a zeroed workspace for one call on the current stream, and the tensor that holds it: cached per device,
+    stream and thread, and a fresh one inside a graph capture, so that calls on two streams or from two threads (whose
+    launches may alternate on one stream), or two captured graphs, never share one."""
     if nbytes == 0:
         return None, None
     if torch._C._cuda_isCurrentStreamCapturing():
         buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     else:
-        buf = _ws_cache.get((device, stream))
+        key = (device, stream, threading.get_ident())
+        buf = _ws_cache.get(key)
         if buf is None or buf.numel() < nbytes:
-            buf = _ws_cache[device, stream] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+            buf = _ws_cache[key] = torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return buf.data_ptr(), buf
 
 

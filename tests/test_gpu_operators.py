@@ -619,3 +619,40 @@ def test_sample_past_one_launch_of_rows():
     """More rows than one set of launches takes."""
     l, u, _ = _lm_logits(1100, 700, 31, bf16=True)
     check_sample(l, u, top_k=_col(1100, [0, 20], torch.int32), top_p=_col(1100, [0.9, 1.0, 0.5]))
+
+
+def test_threads_on_one_stream():
+    """Two threads that call on the same stream, so that their launches alternate: each gets the results it gets alone."""
+    import threading
+    d = _step(T=7)
+    ins = [_step_inputs(d, s) for s in (11, 12)]
+    alone = [_run_step(d, *i) for i in ins]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        for _ in range(30):
+            got = _run_step(d, *ins[k])
+            torch.cuda.synchronize()
+            wrong.extend(n for n in ("x1", "idx", "wt", "token", "prob") if not torch.equal(got[n], alone[k][n]))
+
+    ts = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,N", [(3, 256), (40, 256), (200, 256), (300, 1001)])
+@pytest.mark.parametrize("act", ["gelu", "none"])
+def test_epilogue_bias_off_alignment(bits, M, N, act):
+    """A bias that begins at an odd place of a larger tensor."""
+    ops = _ops()
+    K = 512
+    layer, w = _layer(N, K, bits, 8)
+    A = torch.randn((M, K), device="cuda").to(torch.bfloat16)
+    bias = torch.randn((N + 3,), device="cuda").to(torch.bfloat16)[1:N + 1]
+    call = ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi
+    assert torch.equal(call(A, layer, bias=bias, act=act), call(A, layer, bias=bias.clone(), act=act))
