@@ -1,4 +1,8 @@
 // What a linear's epilogue does with a sum y (fp32): act(y + bias) + residual, rounded once to the output's type.
+// It rides on the products' stores (or on the sums of a split K), so it costs no pass over C: against the plain product
+// 10.1 us for 9.8 (1 row, 5120 x 5120, bias and residual), 28.6 for 28.2 (12 rows, 8-bit, 17408 x 5120, bias and SILU), 18.9
+// for 18.6 (32 rows, 17408 x 5120, bias and GELU_TANH), 155 for 158 of the product with mode 1 (777 rows, 5120 x 17408, bias
+// and residual).
 #pragma once
 #include "common.h"
 

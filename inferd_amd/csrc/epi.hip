@@ -1,5 +1,5 @@
 // The sum of a K split's partials with the linear's epilogue, where the GEMM's own blocks do not join them: rows whose
-// length is no multiple of four in the decode GEMV.
+// length is no multiple of four in the decode GEMV. One pass over S M N floats of at most 16 rows: a launch bounds it.
 #include "epi.h"
 #include "host.h"
 #include "kernels.h"

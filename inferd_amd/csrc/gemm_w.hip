@@ -108,7 +108,9 @@ __device__ __forceinline__ void w_swap32(uint32_t& lo, uint32_t& hi) {
 // The linear's epilogue (p.e) has a form of either kind: kWEpi + class of the activation writes bf16 (the bias 8-byte
 // aligned, and the residual with its rows), kWEpiScalar either type. With every activation in one kernel the epilogues of
 // 192 rows and more spill sums (17 to 104 registers), and past 160 rows the scalar one is too long to be unrolled: it takes
-// tiles of 128 and 160.
+// tiles of 128 and 160 (2048 x 9001 x 5120 with GELU 223.9 us; with a kernel per class and tiles up to 256 223.3, and half a
+// minute more of compiling). 4096 x 17408 x 5120 with bias: 614 us, SILU 623, GELU_TANH 618, GELU 637, the product alone 608:
+// what an activation adds is its instructions, which nothing hides where one wave has a SIMD.
 enum WStore { kWBf16 = 0, kWAdd = 1, kWF32 = 2, kWSwiglu = kModeSwiglu, kWScalar = 4, kWEpiScalar = 5, kWEpi = 6 };
 __host__ __device__ constexpr bool w_scalar(int ST) { return ST == kWScalar || ST == kWEpiScalar; }
 __host__ __device__ constexpr bool w_epi(int ST) { return ST >= kWEpiScalar; }

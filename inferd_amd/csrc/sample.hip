@@ -294,6 +294,15 @@ __device__ __attribute__((noinline)) void row_sample(RowLds& s, const SampleArgs
 // The estimate only chooses what is listed: k_sample_draw checks that the exact border lies inside. Where it does not, or
 // the list is full (thousands of equal logits at the border, top_p within 4e-4 of 1 on a flat row), top_k is past 1024 or
 // the maximum infinite, it takes the one-block path above. Both give the same token.
+//
+// What bounds it, us per kernel (max / border / collect / draw; fp32 logits unless noted):
+//   1 row of 248320, top-k and top-p       3.7 / 3.1 / 5.0 / 8.8   dependent launches, each a chain of memory latencies
+//   7 rows of 50021 (bf16), min-p          2.6 / -   / 5.9 / 7.4   the same
+//   32 rows of 151936, filters mixed       6.5 / 5.5 / 12 / 14     the same, and the longest row's draw
+//   128 rows of 248320, top-p              24  / 23  / 52 / 18     max reads at 5.3 TB/s; border and collect read again (from the
+//                                          last cache) and issue: some 12 and 35 vector instructions per logit, 20 us of
+//                                          collect's for the 64-bit exponentials
+// One block per row took 401, 46, 436 and 928 us a call; these launches 20, 15, 37 and 110.
 constexpr int kTile = 1024, kList = 4096, kMaxK = 1024, kBins = 4096;
 constexpr float kBinScale = 128.f;  // bins per unit of (max - l) / temperature
 constexpr int kRowsPerLaunch = 512, kSomeWaves = 8, kCollect = 768;
