@@ -36,7 +36,8 @@ __device__ __forceinline__ float act_gelu_tanh(float x) {
   return x * epi_rcp(1.f + epi_exp2(x * __builtin_fmaf(x * x, -0.102943240f, -2.30220819f)));
 }
 // x Phi(x): with t = 1 / (1 + p z), z = |x| / sqrt 2, Phi(-|x|) = exp(-z^2) t (a1 + t (a2 + ..)) / 2 to 7.5e-8
-// (Abramowitz and Stegun 7.1.26)
+// (Abramowitz and Stegun 7.1.26). The error falls with exp(-z^2): relative to the value 5e-5 at x = -3, 1.6e-3 at -5, 3.6e-3 at -6
+// (half a bf16 step is 3.9e-3, and the value 6e-9).
 __device__ __forceinline__ float act_gelu(float x) {
   const float t = epi_rcp(__builtin_fmaf(fabsf(x), 0.3275911f * 0.707106781f, 1.f));
   float q = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
