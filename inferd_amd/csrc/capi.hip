@@ -393,9 +393,14 @@ int check_epi(const void* A, int lda, const void* wt, int N, int K, const uint16
   IFD_CHECK(!workspace || aligned(workspace, 16), "workspace must be 16-byte aligned");
   if (res) {
     const char *c = (const char*)C, *r = (const char*)res;
-    const size_t ce = ((size_t)(M - 1) * ldc + N) * (out_f32 ? 4 : 2), re = ((size_t)(M - 1) * ldr + N) * 2;
-    IFD_CHECK((c == r && ldc == ldr && !out_f32) || c + ce <= r || r + re <= c,
-              "the residual overlaps C without being C itself");
+    const size_t esz = out_f32 ? 4 : 2, pitch = ldc * esz;
+    const size_t ce = (M - 1) * pitch + N * esz, re = ((size_t)(M - 1) * ldr + N) * 2;
+    bool apart = c + ce <= r || r + re <= c;
+    if (!apart && pitch == (size_t)ldr * 2) {  // other columns of the same rows
+      const size_t d = r >= c ? (r - c) % pitch : (pitch - (c - r) % pitch) % pitch;
+      apart = d >= N * esz && d + (size_t)N * 2 <= pitch;
+    }
+    IFD_CHECK(apart || (c == r && ldc == ldr && !out_f32), "the residual overlaps C without being C itself");
   }
   return IFD_OK;
 }

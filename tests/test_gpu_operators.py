@@ -656,3 +656,22 @@ def test_epilogue_bias_off_alignment(bits, M, N, act):
     bias = torch.randn((N + 3,), device="cuda").to(torch.bfloat16)[1:N + 1]
     call = ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi
     assert torch.equal(call(A, layer, bias=bias, act=act), call(A, layer, bias=bias.clone(), act=act))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,swap", [(1, False), (3, False), (3, True), (40, False), (150, True)])
+def test_epilogue_residual_in_other_columns_of_the_same_rows(bits, M, swap):
+    ops = _ops()
+    layer, _ = _layer(256, 512, bits, 3)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    A = torch.randn((M, 512), device="cuda", generator=g).to(torch.bfloat16)
+    buf = torch.randn((M, 512 + 8), device="cuda", generator=g).to(torch.bfloat16)
+    c, r = (264, 0) if swap else (0, 264)
+    call = ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi
+    want = call(A, layer, act="silu", residual=buf[:, r:r + 256].clone())
+    res = buf[:, r:r + 256].clone()
+    call(A, layer, act="silu", residual=buf[:, r:r + 256], C=buf[:, c:c + 256])
+    assert torch.equal(buf[:, c:c + 256], want) and torch.equal(buf[:, r:r + 256], res)
+    if M > 1:
+        with pytest.raises(RuntimeError, match="overlaps"):
+            call(A, layer, act="silu", residual=buf[:, 8:264], C=buf[:, :256])
