@@ -258,12 +258,12 @@ __device__ __forceinline__ void sort_falling(uint32_t (&v)[N]) {
 }
 
 // Whether two fp32 choices, or sums of two, may be in the other order. A sigmoid is off by less than 2^-22 (the exponential's
-// argument and its last place, the reciprocal's), a softmax by less than 2^-19 of itself (21 additions more), the bias's
-// addition and that of a group's two values by 2^-24 of their result; the last four bits of a key hide 2^-19 of a value.
-// Equal infinities are exact.
+// argument and its last place, the reciprocal's), a softmax by less than 2^-19 of the largest one, `top` (21 additions more; the
+// argument's rounding grows with it, but less than the exponential falls); the bias's addition and that of a group's two values
+// by 2^-24 of their result; the last four bits of a key hide 2^-19 of a value. Equal infinities are exact.
 template <bool SOFTMAX, bool KEYS>
-__device__ __forceinline__ bool too_near(float hi, float lo) {
-  const float m = __builtin_fmaf(fabsf(hi) + fabsf(lo), KEYS ? 0x1p-18f : 0x1p-23f, SOFTMAX ? 0x1p-17f : 0x1p-20f);
+__device__ __forceinline__ bool too_near(float hi, float lo, float top) {
+  const float m = __builtin_fmaf(fabsf(hi) + fabsf(lo), KEYS ? 0x1p-18f : 0x1p-23f, SOFTMAX ? 0x1p-16f * top : 0x1p-20f);
   return !(hi - lo > m) && !(hi == lo && fabsf(hi) == INFINITY);
 }
 
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
 #pragma unroll
   for (int i = 0; i < PER; i++) l[i] = fmaxf(l[i], -INFINITY) + 0.f;  // NaN: -infinity; -0: +0
   const bool scores = p.bias != nullptr || (p.groups > 1 && GTOP == 2);
-  float mx = 0.f, s[PER];
+  float mx = 0.f, top = 1.f, s[PER];  // the largest logit and score
   if constexpr (SOFTMAX) {
     mx = l[0];
 #pragma unroll
@@ -315,6 +315,7 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
       const float rs = mx == -INFINITY ? 0.f : __builtin_amdgcn_rcpf(all_sum_f<LPR>(sum));
 #pragma unroll
       for (int i = 0; i < PER; i++) s[i] *= rs;
+      top = rs;
     } else {
 #pragma unroll
       for (int i = 0; i < PER; i++) s[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(l[i] * -1.44269504f));
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
     }
     if (p.bias || GTOP == 2) {  // a group that stays against those that do not
       const float out = all_max_f<LPR>(g < p.groups && rank >= p.topk_groups ? mine : -INFINITY);
-      redo_me = g < p.groups && rank < p.topk_groups && p.topk_groups < p.groups && too_near<SOFTMAX, false>(mine, out);
+      redo_me = g < p.groups && rank < p.topk_groups && p.topk_groups < p.groups && too_near<SOFTMAX, false>(mine, out, top);
     }
     const uint64_t keep = __ballot(g < p.groups && rank < p.topk_groups) >> (r * LPR);
     int eg = e0 / gs, left = gs - e0 % gs;
@@ -423,26 +424,40 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
       w = y < 0 ? z * q : q;
     }
   }
-  double sum = 1.0;
-  if constexpr (SOFTMAX)
-    if (p.bias || !p.norm) {
-      double all = 0;
+  // the softmax's sum in 64 bits, which divides the scores (and cancels where the weights are divided by the picks' own sum)
+  auto total = [&] {
+    double all = 0;
 #pragma unroll
-      for (int i = 0; i < PER; i++) all += l[i] == -INFINITY ? 0.0 : l[i] == mx ? 1.0 : exp_neg((double)l[i] - (double)mx);
-      sum = row_sum_f64(all);
-      if constexpr (LPR >= 32) sum += __shfl_xor(sum, 16, 64);
-      if constexpr (LPR == 64) sum += __shfl_xor(sum, 32, 64);
-      w = sum > 0 ? w / sum : 0.0;
+    for (int i = 0; i < PER; i++) all += l[i] == -INFINITY ? 0.0 : l[i] == mx ? 1.0 : exp_neg((double)l[i] - (double)mx);
+    all = row_sum_f64(all);
+    if constexpr (LPR >= 32) all += __shfl_xor(all, 16, 64);
+    if constexpr (LPR == 64) all += __shfl_xor(all, 32, 64);
+    return all;
+  };
+  if constexpr (SOFTMAX)
+    if (!p.norm) {
+      const double all = total();
+      w = all > 0 ? w / all : 0.0;
     }
   int at = c;  // the place of this lane's expert among the few
   if (p.bias || !BF16) {
+    // logits themselves: only equal keys are in doubt
+    auto doubt = [&](uint32_t hi, uint32_t lo) {
+      return lo != 0 && (p.bias ? too_near<SOFTMAX, true>(key_value(hi), key_value(lo), top) : hi == lo);
+    };
     const uint32_t after = (uint32_t)__shfl_down((int)picked, 1, 64);
-    const bool near = c + 1 < few && after != 0 && too_near<SOFTMAX, true>(key_value(picked), key_value(after));
-    // the one behind the few
-    const uint32_t beyond = few > p.k ? m : rest;
-    if (beyond != 0) redo_me |= too_near<SOFTMAX, true>(key_value(last), key_value(beyond));
+    const bool near = c + 1 < few && doubt(picked, after);
+    redo_me |= doubt(last, few > p.k ? m : rest);  // the one behind the few
     if (__ballot(near)) {
-      const double mine = p.bias ? w + (double)order_value(p.bias[who]) : y;
+      double mine = y;
+      if (p.bias) {
+        mine = w;
+        if (SOFTMAX && p.norm) {
+          const double all = total();
+          mine = all > 0 ? w / all : 0.0;
+        }
+        mine += (double)order_value(p.bias[who]);
+      }
       at = 0;
       for (int j = 0; j < few; j++) {
         const double x = __shfl(mine, r * LPR + j, 64);
@@ -455,7 +470,7 @@ __global__ __launch_bounds__(256) void k_moe_route_fast(RouteExArgs p) {
   auto redo_row = [&](int rr) { return (redo >> (rr * LPR) & kLanes) != 0; };
   const bool live = c < few && picked != 0 && at < p.k && t < p.T && !redo_row(r);
   if (p.norm) {
-    sum = row_sum_f64(c < few && at < p.k ? w : 0.0);
+    double sum = row_sum_f64(c < few && at < p.k ? w : 0.0);
     if constexpr (LPR >= 32) sum += __shfl_xor(sum, 16, 64);  // the 17th lane's
     w = sum > 0 ? w / sum : 0.0;
   }

@@ -675,3 +675,15 @@ def test_epilogue_residual_in_other_columns_of_the_same_rows(bits, M, swap):
     if M > 1:
         with pytest.raises(RuntimeError, match="overlaps"):
             call(A, layer, act="silu", residual=buf[:, 8:264], C=buf[:, :256])
+
+
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k,groups,keep,top", [(256, 8, 8, 4, 2), (96, 16, 1, 1, 1), (512, 10, 4, 3, 1)])
+@pytest.mark.parametrize("spread", [1e-2, 1e-4, 1e-6])
+def test_route_of_choices_close_together(norm, score, E, k, groups, keep, top, spread):
+    """Scores and biases apart by less than fp32 tells, up to all of a token's."""
+    g = torch.Generator(device="cuda").manual_seed(E + k)
+    l = 0.5 + spread * torch.randn((40, E), device="cuda", generator=g)
+    bias = 0.1 * spread * torch.randn((E,), device="cuda", generator=g)
+    check_route(l, E, k, score=score, bias=bias, groups=groups, topk_groups=keep, group_top=top, norm=norm)
