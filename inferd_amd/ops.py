@@ -34,9 +34,10 @@ _ws_cache: dict = {}
 
 
 def workspace(nbytes: int, device) -> torch.Tensor:
-    """A cached uint8 device buffer of at least nbytes (grown on demand), reused across calls on one stream.
-    Allocated zeroed: a workspace's leading counters must start at zero, and the library keeps them there."""
-    key = str(device)
+    """A cached uint8 device buffer of at least nbytes (grown on demand), reused across a thread's calls on one stream (two
+    threads' launches may alternate on it). Allocated zeroed: a workspace's leading counters must start at zero, and the
+    library keeps them there."""
+    key = (str(device), threading.get_ident())
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)

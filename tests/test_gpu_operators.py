@@ -634,7 +634,7 @@ def test_threads_on_one_stream():
         for _ in range(30):
             got = _run_step(d, *ins[k])
             torch.cuda.synchronize()
-            wrong.extend(n for n in ("x1", "idx", "wt", "token", "prob") if not torch.equal(got[n], alone[k][n]))
+            wrong.extend(n for n in alone[k] if not torch.equal(got[n], alone[k][n]))
 
     ts = [threading.Thread(target=work, args=(k,)) for k in range(2)]
     for t in ts:
@@ -687,3 +687,26 @@ def test_route_of_choices_close_together(norm, score, E, k, groups, keep, top, s
     l = 0.5 + spread * torch.randn((40, E), device="cuda", generator=g)
     bias = 0.1 * spread * torch.randn((E,), device="cuda", generator=g)
     check_route(l, E, k, score=score, bias=bias, groups=groups, topk_groups=keep, group_top=top, norm=norm)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("M,N,K", [(16, 131201, 1536), (3, 7409, 1536), (12, 1050, 2304), (9, 131071, 1536), (1, 5, 5120)])
+def test_epilogue_of_split_rows_of_any_length(bits, M, N, K):
+    """Partial sums joined in the GEMV and, past its counters' columns, by a launch: the plain product's fp32 sums bit for bit,
+    and what the epilogue makes of them."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(N)
+    wq = torch.randint(-2 ** 31, 2 ** 31 - 1, (N, K * bits // 32), device="cuda", dtype=torch.int32, generator=g)
+    s = (0.01 * torch.randn((N, K // 64), device="cuda", generator=g)).to(torch.bfloat16)
+    b = (0.01 * torch.randn((N, K // 64), device="cuda", generator=g)).to(torch.bfloat16)
+    layer = (ops.pack_t64 if bits == 4 else ops.pack_t64x8)(ops.QLinear(wq, s, b, N, K, False, bits))
+    A = torch.randn((M, K), device="cuda", generator=g).to(torch.bfloat16)
+    y = (ops.gemm_t64 if bits == 4 else ops.gemm_t64x8)(A, layer, mode=2)
+    call = ops.gemm_t64_epi if bits == 4 else ops.gemm_t64x8_epi
+    assert torch.equal(call(A, layer, fp32=True), y)
+    big = torch.full((M, N + 3), 7.0, device="cuda")  # rows further apart, not 16-byte aligned
+    bias = torch.randn((N,), device="cuda", generator=g).to(torch.bfloat16)
+    res = torch.randn((M, N), device="cuda", generator=g).to(torch.bfloat16)
+    call(A, layer, bias=bias, act="relu", residual=res, C=big[:, :N])
+    assert torch.equal(big[:, :N], torch.relu(y + bias.float()) + res.float())
+    assert bool((big[:, N:] == 7).all())
