@@ -228,7 +228,7 @@ int ifd_gemm_t64x8_w8a8(const int8_t* U, const float* XS, int per_token, const v
  *   RELU max(y, 0); SILU y / (1 + exp(-y)); GELU y Phi(y) (Phi the normal distribution's); GELU_TANH
  *   y / (1 + exp(-2 sqrt(2 / pi) (y + 0.044715 y^3))), the tanh form of the same.
  * K % 256 == 0 (T64) or K % 64 == 0 (T64x8), lda % 8 == 0; A and wt 16-byte aligned; any N and ldc >= N; C must not
- * overlap A, wt or the bias. Workspace as for the product. Past 16 rows A and W are to span less than 2 GiB each
+ * overlap A, wt or the bias. Workspace as for the product, by queries of their own. Past 16 rows A and W are to span less than 2 GiB each
  * (IFD_ERR_UNSUPPORTED else). */
 enum { IFD_ACT_NONE = 0, IFD_ACT_RELU = 1, IFD_ACT_SILU = 2, IFD_ACT_GELU = 3, IFD_ACT_GELU_TANH = 4 };
 size_t ifd_gemm_t64_epi_workspace(int M, int N, int K);

@@ -406,7 +406,10 @@ int check_epi(const void* A, int lda, const void* wt, int N, int K, const uint16
 }
 }  // namespace
 
-size_t ifd_gemm_t64_epi_workspace(int M, int N, int K) { return K % 256 ? 0 : ifd_gemm_t64_workspace(M, N, K); }
+size_t ifd_gemm_t64_epi_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 256) return 0;
+  return M <= 16 ? with_header(qmv_t_workspace(M, N, K, kModeEpi)) : ifd_gemm_t64_workspace(M, N, K);
+}
 
 int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
                      const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace, size_t ws_bytes,
@@ -421,7 +424,10 @@ int ifd_gemm_t64_epi(const void* A, int lda, const void* wt, int N, int K, const
   return launch_gemm_t((const uint16_t*)A, lda, wt, N, K, C, ldc, M, kModeEpi, w.body, w.bytes, S(stream), &e);
 }
 
-size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K) { return ifd_gemm_t64x8_workspace(M, N, K); }
+size_t ifd_gemm_t64x8_epi_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K % 64) return 0;
+  return t64x8_qmv(M, K) ? with_header(qmv_t_workspace(M, N, K, kModeEpi, 8)) : ifd_gemm_t64x8_workspace(M, N, K);
+}
 
 int ifd_gemm_t64x8_epi(const void* A, int lda, const void* wt, int N, int K, const uint16_t* bias, int act,
                        const void* res, int ldr, void* C, int ldc, int M, int out_f32, void* workspace,

@@ -8,6 +8,9 @@
 
 namespace ifd {
 
+// A row of a K split's partials in the decode GEMV with an epilogue: whole 16-byte quads.
+__host__ __device__ inline int epi_part_row(int N) { return (N + 3) / 4 * 4; }
+
 enum EpiAct { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
 
 struct Epi {

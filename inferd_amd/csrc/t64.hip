@@ -266,7 +266,8 @@ __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
       const int row = 8 * (r / 4) + 4 * h + (r % 4);
       if (row < M)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[r]),  rs,
-                                              (int)((((size_t)blockIdx.y * M + row) * p.N + gcol) * 4), 0, kSc1);
+                                              (int)((((size_t)blockIdx.y * M + row) * (EPI ? epi_part_row(p.N) : p.N) + gcol) * 4), 0,
+                                              kSc1);
     }
   }
   if (!p.cnt) return;
@@ -283,8 +284,9 @@ __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
   __syncthreads();
   if (!s_last) return;
   const int S = (int)gridDim.y;
-  const size_t mn = (size_t)M * p.N;
-  // four columns of one row per thread and pass (16-byte partial loads, N % 4 == 0), the loads of kFixB splits in
+  const int pn = EPI ? epi_part_row(p.N) : p.N;
+  const size_t mn = (size_t)M * pn;
+  // four columns of one row per thread and pass (16-byte partial loads of rows that are a multiple of 4 long), the loads of kFixB splits in
   // flight at once (their registers count against the occupancy the stream needs), summed in split order
   auto sum4 = [&](size_t o) {
     float4 acc4 = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -311,11 +313,12 @@ __global__ __launch_bounds__(256, 2) void k_qmv_t(QmvTArgs p) {
     if (!p.sw_half) {
       const int c = (int)blockIdx.x * 128 + c4, cl = c - 32 * gb0;  // global, and the linear's column
       if (cl >= Nl) continue;
-      const float4 v = sum4((size_t)row * p.N + c);
+      const float4 v = sum4((size_t)row * pn + c);
       const size_t o = (size_t)row * ldcl + cl;
-      if constexpr (EPI) {  // N % 4 == 0
+      if constexpr (EPI) {
         float x[4] = {v.x, v.y, v.z, v.w};
-        epi_store(p.e, Cl, o, row, cl, 4, x);
+        if (cl + 4 <= Nl) epi_store(p.e, Cl, o, row, cl, 4, x);
+        else epi_store(p.e, Cl, o, row, cl, Nl - cl, x);
         continue;
       }
       // a linear of the multi-linear launch may end inside the quad (its N need not be a multiple of 4)
@@ -355,17 +358,17 @@ static TPlan qmv_t_plan(int M, int N, int K, int bits = 4) {
   return TPlan{(G + gps - 1) / gps, gps};
 }
 
-// The in-kernel fixup applies with counters for every tile and rows of whole 16-byte partial quads (N % 4 == 0); the
-// SwiGLU pairing needs gate and up halves of whole 128-column tiles.
+// The in-kernel fixup applies with counters for every tile and rows of whole 16-byte partial quads (N % 4 == 0, or the
+// epilogue's, whose partial rows are padded: 3 x 7409 x 1536 8.8 us, with a launch of its own for the sums 12.3); the SwiGLU pairing needs gate and up halves of whole 128-column tiles.
 static bool qmv_t_fixup(int N, int mode, int S) {
   const int tiles = (t64_bands(N) + 3) / 4;
-  if (S <= 1 || tiles > kWsCounters || N % 4) return false;
+  if (S <= 1 || tiles > kWsCounters || (N % 4 && mode != kModeEpi)) return false;
   return mode != kModeSwiglu || (N % 256 == 0);
 }
 
 size_t qmv_t_workspace(int M, int N, int K, int mode, int bits) {
   if (M > 16) return 0;
-  return epilogue_ws_bytes(qmv_t_plan(M, N, K, bits).S, M, N, mode);
+  return epilogue_ws_bytes(qmv_t_plan(M, N, K, bits).S, M, mode == kModeEpi ? epi_part_row(N) : N, mode);
 }
 
 template <int BITS, bool A8 = false>
@@ -376,7 +379,7 @@ static int launch_qmv_t_bits(const uint16_t* A, int lda, const void* wt, int N, 
   if (M > 16) return fail(IFD_ERR_UNSUPPORTED, "T64 decode kernel takes M <= 16");
   if (K % (kGroup * kTB)) return fail(IFD_ERR_ARG, "T64 decode needs K %% %d == 0 (K=%d)", kGroup * kTB, K);
   const TPlan pl = qmv_t_plan(M, N, K, BITS);
-  const size_t need = epilogue_ws_bytes(pl.S, M, N, mode);
+  const size_t need = qmv_t_workspace(M, N, K, mode, BITS);
   if (need > ws_bytes || (need && !ws))
     return fail(IFD_ERR_WORKSPACE, "qmv_t64 needs %zu bytes of workspace, got %zu", need, ws_bytes);
   const bool fix = cnt && qmv_t_fixup(N, mode, pl.S);
