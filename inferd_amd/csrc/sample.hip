@@ -293,7 +293,8 @@ __device__ __attribute__((noinline)) void row_sample(RowLds& s, const SampleArgs
 //                    sums, then its place.
 // The estimate only chooses what is listed: k_sample_draw checks that the exact border lies inside. Where it does not, or
 // the list is full (thousands of equal logits at the border, top_p within 4e-4 of 1 on a flat row), top_k is past 1024 or
-// the maximum infinite, it takes the one-block path above. Both give the same token.
+// the maximum infinite, it takes the one-block path above. Both give the same token. A row no longer than the list is its own
+// list, and k_sample_draw alone does it.
 //
 // What bounds it, us per kernel (max / border / collect / draw; fp32 logits unless noted):
 //   1 row of 248320, top-k and top-p       3.7 / 3.1 / 5.0 / 8.8   dependent launches, each a chain of memory latencies
@@ -725,7 +726,8 @@ __device__ __forceinline__ void sort_lanes(uint64_t& v, uint64_t& w) {
   merge_lanes<64, 32>(v, w);
 }
 
-template <bool BF16>
+// DIRECT: the list is the row itself (V <= kList), and there is no other launch.
+template <bool BF16, bool DIRECT>
 __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, SampleWs ws) {
   __shared__ DrawLds s;
   constexpr int PER = kList / kRowThreads;
@@ -733,11 +735,22 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
   const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   // loads that depend on nothing, together (a row's draw is a chain of memory latencies)
   const RowPar r = row_par(p, t);
-  const RowInfo in = *ws.info(t);
-  const float tile_max = tid < ws.tiles ? ws.tmax(t)[tid] : -INFINITY;
-  const uint64_t tile_sum = tid < ws.tiles ? ws.tsum(t)[tid] : 0;
-  uint64_t a[PER], f[PER];
-  a[0] = ws.list(t)[tid];
+  RowInfo in{};
+  float tile_max = -INFINITY;
+  uint64_t tile_sum = 0, a[PER], f[PER];
+  if constexpr (DIRECT) {
+#pragma unroll
+    for (int q = 0; q < PER; q++) {
+      const int i = kRowThreads * q + tid;
+      const float l = load_logit<BF16>(p, t, min(i, p.V - 1));
+      a[q] = (uint64_t)~order_key(i < p.V ? l : -INFINITY) << 32 | (uint32_t)i;
+      tile_max = fmaxf(tile_max, l);
+    }
+  } else {
+    in = *ws.info(t);
+    if (tid < ws.tiles) tile_max = ws.tmax(t)[tid], tile_sum = ws.tsum(t)[tid];
+    a[0] = ws.list(t)[tid];
+  }
   const double u = row_u(p, t);
   float mx = dpp_max_f(tile_max);
   if (lane == 0) s.s[tid >> 6] = mx;
@@ -745,7 +758,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kRowThreads / 64; i++) mx = fmaxf(mx, s.s[i]);
-  const int kind = row_kind(r, p.V, mx);
+  const int kind = DIRECT && mx < INFINITY && r.k < p.V && !r.greedy && mx > -INFINITY ? kTopK : row_kind(r, p.V, mx);
   auto done = [&](int token, float prob) {
     p.token[t] = token;
     if (p.prob) p.prob[t] = prob;
@@ -755,6 +768,14 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
     return;
   }
   if (kind == kGreedy) {  // the first tile with the maximum, and its place there
+    if constexpr (DIRECT) {
+#pragma unroll
+      for (int q = PER - 1; q >= 0; q--)
+        if (entry_logit(a[q]) == mx) atomicMin(&s.at, (int)(uint32_t)a[q]);
+      __syncthreads();
+      if (tid == 0) done(s.at, 1.f);
+      return;
+    }
     if (tile_max == mx) atomicMin(&s.at, tid);
     __syncthreads();
     const int first = s.at * kTile;
@@ -767,7 +788,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
     if (tid == 0) done(s.at, 1.f);
     return;
   }
-  const int n = (int)min(in.n, (uint32_t)kList + 1);
+  const int n = DIRECT ? p.V : (int)min(in.n, (uint32_t)kList + 1);
   if (kind == kTopK && n <= 64) {  // a short list by one wave: sorted, cut, and sorted again into the vocabulary's order
     if (tid >= 64) return;
     uint64_t e = lane < n ? a[0] : ~0ull, w = lane < n ? weight(entry_logit(a[0]), mx, r.rt) : 0;
@@ -788,18 +809,19 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
   // what is kept: the prefix of the order up to the entry `border`, as far as it has min_p
   uint64_t border = ~0ull;
   int sub[PER];
-  if (listed && kind != kFull) {
-    // the list in registers, over 512 sub-bins of its range of logits
+  if (listed && (DIRECT || kind != kFull)) {
+    // the list in registers (what has a weight), over 512 sub-bins of its range of logits
     float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
     for (int q = 0; q < PER; q++) {
       const int i = kRowThreads * q + tid;
-      if (q > 0) a[q] = 0;
+      if (!DIRECT && q > 0) a[q] = 0;
       f[q] = 0;
       if (kRowThreads * q >= n) continue;
-      if (q > 0) a[q] = ws.list(t)[min(i, n - 1)];
+      if (!DIRECT && q > 0) a[q] = ws.list(t)[min(i, n - 1)];
       const float l = entry_logit(a[q]);
-      if (i < n) f[q] = weight(l, mx, r.rt), lo = fminf(lo, l), hi = fmaxf(hi, l);
+      if (i < n) f[q] = weight(l, mx, r.rt);
+      if (f[q]) lo = fminf(lo, l), hi = fmaxf(hi, l);
     }
     lo = -dpp_max_f(-lo), hi = dpp_max_f(hi);
     if (lane == 0) s.npart[tid >> 6] = __float_as_uint(lo), s.s[tid >> 6] = hi;
@@ -811,30 +833,30 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
 #pragma unroll
     for (int q = 0; q < PER; q++) {
       sub[q] = -1;
-      if (kRowThreads * q + tid < n) {
+      if (f[q]) {
         sub[q] = min((int)((hi - entry_logit(a[q])) * sc), kSub - 1);
         atomicAdd(&s.f.n[sub[q]], 1u);
-        if (f[q]) atomicAdd((unsigned long long*)&s.f.w[sub[q]], (unsigned long long)f[q]);
+        atomicAdd((unsigned long long*)&s.f.w[sub[q]], (unsigned long long)f[q]);
       }
     }
     __syncthreads();
     const uint64_t own_w = s.f.w[tid];
     const uint32_t own_n = s.f.n[tid];
-    const uint32_t k = (uint32_t)min(r.k, n);
     uint64_t bw = own_w, W;
     uint32_t bn = own_n, Nn;
     draw_scan(s, bw, bn, W, Nn);  // this thread's sub-bin: what comes before it
-    if (tid < ws.tiles) s.f.tile[tid] = kind == kTopP ? tile_sum : 0;
+    const uint32_t k = min((uint32_t)r.k, Nn);
+    if (tid < ws.tiles) s.f.tile[tid] = !DIRECT && kind == kTopP ? tile_sum : 0;
     // The border by count (top-k: the k-th entry, or the last), then by weight (the first entry at which the sum reaches want, `base`
     // before the list): its sub-bin, and there, among few, the entry.
 #pragma clang loop unroll(disable)
     for (int step = 0; step < 2; step++) {
       const bool by_count = step == 0;
       if (by_count ? kind != kTopK : r.top_p >= 1.0) continue;
-      const uint64_t base = kind == kTopP ? in.before : 0;
+      const uint64_t base = !DIRECT && kind == kTopP ? in.before : 0;
       double want = 0;
       if (!by_count) {
-        want = r.top_p * (double)(kind == kTopK ? s.upto : in.all);
+        want = r.top_p * (double)(kind == kTopK ? s.upto : DIRECT ? W : in.all);
         // the border lies above what is listed, or below
         listed = (base == 0 || (double)base < want) && (double)(base + W) >= want;
         if (!listed) break;
@@ -887,7 +909,7 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < PER; q++)
-      if (sub[q] >= 0 && a[q] <= border && f[q] && f[q] >= r.min_w)
+      if (sub[q] >= 0 && a[q] <= border && f[q] >= r.min_w)
         atomicAdd((unsigned long long*)&s.f.tile[(uint32_t)a[q] / kTile], (unsigned long long)f[q]);
   } else if (listed) {
     if (tid < ws.tiles) s.f.tile[tid] = tile_sum;
@@ -938,10 +960,16 @@ __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SampleArgs p, Sampl
   if (fat && at == s.at) done(at, (float)((double)fat / (double)total));
 }
 
-size_t sample_workspace(int T, int V) { return (size_t)std::min(T, kRowsPerLaunch) * sample_ws(V).row; }
+size_t sample_workspace(int T, int V) { return V <= kList ? 0 : (size_t)std::min(T, kRowsPerLaunch) * sample_ws(V).row; }
 
 template <bool BF16>
 static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream_t st) {
+  // a row that fits the list: one launch (us, against the four: 4 x 4000 top-p 14.6 for 24.0, 17 x 1455 mixed 14.4 for 25.4,
+  // 110 x 4079 min-p 11.6 for 15.2, 1000 x 4096 top-p 64 for 83)
+  if (a.V <= kList) {
+    hipLaunchKernelGGL((k_sample_draw<BF16, true>), dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
+    return check_launch("sample");
+  }
   const auto blocks = [&](int waves) { return (ws.tiles + waves - 1) / waves; };
   // a wave per tile where that does not fill the device; past it fewer blocks, which set up or join a histogram each (128 rows
   // of 248320: 512 / 768 / 1024 / 2048 blocks of k_sample_collect 122 / 116 / 118 / 122 us a call)
@@ -950,7 +978,7 @@ static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream
   hipLaunchKernelGGL(k_sample_max<BF16>, dim3(blocks(4), a.T), dim3(256), 0, st, a, ws);
   if (a.top_k || a.top_p) hipLaunchKernelGGL(k_sample_border<BF16>, some(512), some_threads, 0, st, a, ws);
   hipLaunchKernelGGL(k_sample_collect<BF16>, some(kCollect), some_threads, 0, st, a, ws);
-  hipLaunchKernelGGL(k_sample_draw<BF16>, dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
+  hipLaunchKernelGGL((k_sample_draw<BF16, false>), dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
   return check_launch("sample");
 }
 
@@ -959,11 +987,13 @@ int launch_sample(const void* logits, int logits_bf16, int T, int V, int ld, con
                   size_t ws_bytes, hipStream_t st) {
   SampleWs ws = sample_ws(V);
   ws.base = (char*)mem;
-  if (T && (!mem || ws_bytes < sample_workspace(T, V)))
-    return fail(IFD_ERR_WORKSPACE, "sample needs %zu bytes of workspace, got %zu", sample_workspace(T, V), ws_bytes);
-  for (int t = 0; t < T; t += kRowsPerLaunch) {
+  const size_t need = sample_workspace(T, V);
+  if (need && (!mem || ws_bytes < need))
+    return fail(IFD_ERR_WORKSPACE, "sample needs %zu bytes of workspace, got %zu", need, ws_bytes);
+  const int step = need ? kRowsPerLaunch : T;
+  for (int t = 0; t < T; t += step) {
     auto off = [&](auto* q) { return q ? q + t : q; };
-    const SampleArgs a{(const char*)logits + (size_t)t * ld * (logits_bf16 ? 2 : 4), std::min(T - t, kRowsPerLaunch), V, ld,
+    const SampleArgs a{(const char*)logits + (size_t)t * ld * (logits_bf16 ? 2 : 4), std::min(T - t, step), V, ld,
                        off(temperature), off(top_k), off(top_p), off(min_p), off(u), off(token), off(prob)};
     IFD_TRY(logits_bf16 ? launch_sample_rows<true>(a, ws, st) : launch_sample_rows<false>(a, ws, st));
   }

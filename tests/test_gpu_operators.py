@@ -710,3 +710,22 @@ def test_epilogue_of_split_rows_of_any_length(bits, M, N, K):
     call(A, layer, bias=bias, act="relu", residual=res, C=big[:, :N])
     assert torch.equal(big[:, :N], torch.relu(y + bias.float()) + res.float())
     assert bool((big[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("V", [64, 65, 512, 513, 2047, 4095, 4096, 4097, 8192])
+def test_sample_of_short_rows(V, bf16):
+    """Around the lengths at which a row is its own list: every filter, rows of a few and of all weights."""
+    T = 40
+    l, u, _ = _lm_logits(T, V, V, bf16)
+    l[3:6] *= 1e-3  # flat
+    l[6:9] *= 40  # a few tokens have weights
+    l[9, V // 3:] = -math.inf
+    l[10, 1:] = math.nan
+    l[11] = torch.finfo(l.dtype).min
+    l[12, 5] = math.inf
+    l[13] = -math.inf
+    for kw in (dict(), dict(top_k=_col(T, [1, 17, V - 1, V, 2000, 0], torch.int32)), dict(top_p=_col(T, [0.9, 0.1, 0.0, 1.0, 0.9999])),
+               dict(min_p=_col(T, [0.1, 1e-9])),
+               dict(top_k=_col(T, [60, V // 2, 3], torch.int32), top_p=_col(T, [0.8, 0.95]), min_p=_col(T, [0.0, 0.01]))):
+        check_sample(l, u, temperature=_col(T, [1.0, 0.3, 0.0, 2.0]), **kw)
