@@ -990,8 +990,8 @@ int launch_sample(const void* logits, int logits_bf16, int T, int V, int ld, con
   const size_t need = sample_workspace(T, V);
   if (need && (!mem || ws_bytes < need))
     return fail(IFD_ERR_WORKSPACE, "sample needs %zu bytes of workspace, got %zu", need, ws_bytes);
-  const int step = need ? kRowsPerLaunch : T;
-  for (int t = 0; t < T; t += step) {
+  const int step = need ? kRowsPerLaunch : 1 << 20;  // (a grid holds less than 2^32 threads)
+  for (int t = 0; t < T; t += std::min(step, T - t)) {
     auto off = [&](auto* q) { return q ? q + t : q; };
     const SampleArgs a{(const char*)logits + (size_t)t * ld * (logits_bf16 ? 2 : 4), std::min(T - t, step), V, ld,
                        off(temperature), off(top_k), off(top_p), off(min_p), off(u), off(token), off(prob)};
