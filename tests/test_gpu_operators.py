@@ -713,7 +713,7 @@ def test_epilogue_of_split_rows_of_any_length(bits, M, N, K):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
-@pytest.mark.parametrize("V", [64, 65, 512, 513, 2047, 4095, 4096, 4097, 8192])
+@pytest.mark.parametrize("V", [64, 65, 512, 513, 2047, 4095, 4096, 4097, 6007, 8192, 8193])
 def test_sample_of_short_rows(V, bf16):
     """Around the lengths at which a row is its own list: every filter, rows of a few and of all weights."""
     T = 40
