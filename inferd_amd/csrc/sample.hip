@@ -965,7 +965,7 @@ size_t sample_workspace(int T, int V) { return V <= kList ? 0 : (size_t)std::min
 template <bool BF16>
 static int launch_sample_rows(const SampleArgs& a, const SampleWs& ws, hipStream_t st) {
   // a row that fits the list: one launch (us, against the four: 4 x 4000 top-p 14.6 for 24.0, 17 x 1455 mixed 14.4 for 25.4,
-  // 110 x 4079 min-p 11.6 for 15.2, 1000 x 4096 top-p 64 for 83)
+  // 110 x 4079 min-p 11.6 for 15.2, 1000 x 4096 top-p 64 for 83; with 16 entries per thread for up to 8192 4 x 8192 62 for 24)
   if (a.V <= kList) {
     hipLaunchKernelGGL((k_sample_draw<BF16, true>), dim3(a.T), dim3(kRowThreads), 0, st, a, ws);
     return check_launch("sample");
